@@ -701,6 +701,31 @@ int vhap_adam_step(int n_tensors, float* const* params, const float* const* grad
                    float* const* exp_avg_sq, const int64_t* numel, const int32_t* lr_index,
                    const float* lr_device, int32_t* step_device, float beta1, float beta2, float eps,
                    int call_flags, vhap_stream_t stream);
+/* Global norm of a list of gradients and clipping to a largest norm (vhap_amd/csrc/gradnorm.hip; what torch.nn.utils.clip_grad_norm_ computes):
+ *   norm = (sum |g|^p)^(1/p) over ALL elements of all tensors (norm_kind 1 or 2), or max |g| (VHAP_NORM_INF); summed in 64 bits, in a fixed order
+ *   c = min(1, max_norm / (norm + 1e-6)); a NaN norm makes c NaN; an infinite one makes it 0 (and 0 x infinity NaN)
+ * grads[k]: numel[k] consecutive elements of dtype[k] (VHAP_DTYPE_*; dtype NULL: all float32), aligned to their element; any number of tensors, empty ones
+ * among them; fewer than 2^39 elements in all.  norm: device float, overwritten.  workspace: vhap_grad_norm_workspace_bytes(n_tensors), not shared by
+ * calls in flight at the same time.
+ * vhap_grad_clip: out[k] = round(grads[k] * c) to the same dtype; out[k] is grads[k] itself (in place; a list that is not clipped is then not rewritten) or
+ *   memory of its own: VHAP_E_UNSUPPORTED where a destination overlaps another destination or another tensor's source.  max_norm >= 0.
+ * vhap_adam_step_clipped: vhap_adam_step on round(grads * c), the gradients left as they are, the norm over these n_tensors (2-norm; norm may be NULL):
+ *   the counter is advanced by the call's own launches (no third one).  call_flags as vhap_adam_step.
+ * Lists of at most 32768 elements (by units of 512 a tensor) are one launch, others two, and two more for every further 128 tensors that do not lie one
+ * behind another in memory. */
+#define VHAP_NORM_INF 0
+#define VHAP_DTYPE_F32 0
+#define VHAP_DTYPE_BF16 1
+#define VHAP_DTYPE_F16 2
+size_t vhap_grad_norm_workspace_bytes(int n_tensors);
+int vhap_grad_norm(int n_tensors, const void* const* grads, const int64_t* numel, const int32_t* dtype, int norm_kind,
+                   void* workspace, size_t workspace_bytes, float* norm, vhap_stream_t stream);
+int vhap_grad_clip(int n_tensors, const void* const* grads, void* const* out, const int64_t* numel, const int32_t* dtype,
+                   int norm_kind, float max_norm, void* workspace, size_t workspace_bytes, float* norm, vhap_stream_t stream);
+int vhap_adam_step_clipped(int n_tensors, float* const* params, const float* const* grads, float* const* exp_avg,
+                           float* const* exp_avg_sq, const int64_t* numel, const int32_t* lr_index, const float* lr_device,
+                           int32_t* step_device, float beta1, float beta2, float eps, float max_norm, void* workspace,
+                           size_t workspace_bytes, float* norm, int call_flags, vhap_stream_t stream);
 /* step_device[0] += 1 (one tiny launch): advance the counter at the HEAD of a step, then issue the step's vhap_adam_step calls with
  * VHAP_CALL_ADAM_STEP_ADVANCED. */
 int vhap_adam_advance(int32_t* step_device, vhap_stream_t stream);
@@ -870,6 +895,32 @@ int vhap_nhwc_upsample2_add(const float* skip, const float* low, int N, int H, i
 int vhap_nhwc_maxpool2(const float* in, int N, int H, int W, int C, float* out, vhap_stream_t stream);
 int vhap_nhwc_l2norm(const float* in, long long npix, int C, const float* weight, float eps, float* out, vhap_stream_t stream);
 int vhap_nhwc_add(const float* a, const float* b, const float* c, long long n, float* out, vhap_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (vhap_amd/csrc/mx.hip; host side: vhap_amd/mx.py).  A row of K numbers is Kb = ceil(K / 32) blocks of 32 codes of E2M1
+ * (+-{0, 0.5, 1, 1.5, 2, 3, 4, 6}; two a byte, the even element in the low half) and one byte b a block, the power of two 2^(b - 127) its codes are
+ * multiplied with; b = 255: the block is NaN.  codes [rows, 16 Kb] (16-byte aligned), scales [rows, Kb], both contiguous.  Codes behind K in the last block
+ * are written as zero and read as nothing.  dtype: VHAP_DTYPE_* of the floating-point operand.  Row strides (ldx, ldg) in elements; rows < 2^40, K <= 2^24.
+ *   vhap_mx4_quantize: x [rows, K].  b from the block's largest magnitude (exponent - 2: the largest code in [4, 8), 6 where it would be more), codes to nearest,
+ *     halves to the even code; a block with a NaN or an infinity becomes NaN.
+ *   vhap_mx4_dequantize: out [rows, K] contiguous (float32 and bfloat16 hold every value exactly; float16 rounds, and overflows above 65504).
+ *   vhap_mx4_linear: y [M, N] = x [M, K] W^T + bias; W [N, K] in 4 bits, bias float32 [N] or NULL; x and y of `dtype`, products exact, sums in float32.
+ *   vhap_mx4_linear_input_grad: dx [M, K] = g [M, N] W, N > 0; workspace of _workspace_bytes(M, N, K), partial sums joined in a fixed order;
+ *     VHAP_CALL_MX_ACCUMULATE (float32): dx += .   vhap_mx4_column_sums: out [N] = sum over the M rows of g (the bias' gradient).
+ *   vhap_mx4_matmul: y [M, N] = A [M, K] B [N, K]^T + bias, both in 4 bits; VHAP_CONV_OUT_RELU: ReLU on the way out (a pointwise convolution: M pixels).
+ * Empty results are VHAP_OK without a launch.
+ * ------------------------------------------------------------------------------------------- */
+#define VHAP_CALL_MX_ACCUMULATE 1024
+int vhap_mx4_quantize(const void* x, int dtype, long long ldx, long long rows, int K, uint8_t* codes, uint8_t* scales, vhap_stream_t stream);
+int vhap_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, long long rows, int K, void* out, int dtype, vhap_stream_t stream);
+int vhap_mx4_linear(const void* x, int dtype, long long ldx, long long M, const uint8_t* codes, const uint8_t* scales, long long N, int K,
+                    const float* bias, void* y, vhap_stream_t stream);
+size_t vhap_mx4_linear_input_grad_workspace_bytes(long long M, long long N, int K);
+int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ldg, long long M, const uint8_t* codes, const uint8_t* scales, long long N, int K,
+                               void* workspace, size_t workspace_bytes, void* dx, int call_flags, vhap_stream_t stream);
+int vhap_mx4_column_sums(const void* g, int dtype, long long ldg, long long M, long long N, float* out, vhap_stream_t stream);
+int vhap_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, long long M, const uint8_t* b_codes, const uint8_t* b_scales, long long N, int K,
+                    const float* bias, void* y, int dtype, int call_flags, vhap_stream_t stream);
 
 #ifdef __cplusplus
 }

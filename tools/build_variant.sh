@@ -6,7 +6,7 @@ cd "$(dirname "$0")/.."
 name=$1; src=$2; shift 2
 python -m vhap_amd.build > /dev/null
 obj=vhap_amd/lib/${src%.hip}_$name.o
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wall -Wno-unused-function -Iinclude -Ivhap_amd/csrc "$@" -x hip -c vhap_amd/csrc/$src -o $obj
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -Wall -Wno-unused-function -Iinclude -Ivhap_amd/csrc "$@" -x hip -c vhap_amd/csrc/$src -o $obj
 objs=$(ls vhap_amd/lib/*.o | grep -v "_[a-zA-Z0-9]*\.o$" | grep -v "/${src%.hip}\.o$")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o vhap_amd/lib/libvhap_hip_$name.so $objs $obj
 echo vhap_amd/lib/libvhap_hip_$name.so

@@ -20,7 +20,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 def isa(src, out_dir):
     s = os.path.join(out_dir, os.path.basename(src)[:-4] + ".s")
-    subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", f"-I{ROOT}/include", f"-I{ROOT}/vhap_amd/csrc", "-S",
+    subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", f"-I{ROOT}/include", f"-I{ROOT}/vhap_amd/csrc", "-S",
                     "--cuda-device-only", src, "-o", s], check=True, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
     return s
 

@@ -16,6 +16,7 @@ c_fp = ctypes.c_void_p   # device pointers travel as integers (tensor.data_ptr()
 c_i = ctypes.c_int
 c_sz = ctypes.c_size_t
 c_f = ctypes.c_float
+c_ll = ctypes.c_longlong
 
 # name -> (restype, [argtypes]) ; must list EVERY symbol declared in include/vhap_hip.h
 SIGNATURES = {
@@ -119,6 +120,10 @@ SIGNATURES = {
     "vhap_sum_frames": (c_i, [c_fp, c_i, c_i, c_fp, c_fp]),
     "vhap_adam_step": (c_i, [c_i] + [c_fp] * 8 + [c_f, c_f, c_f, c_i, c_fp]),
     "vhap_adam_advance": (c_i, [c_fp, c_fp]),
+    "vhap_grad_norm_workspace_bytes": (c_sz, [c_i]),
+    "vhap_grad_norm": (c_i, [c_i, c_fp, c_fp, c_fp, c_i, c_fp, c_sz, c_fp, c_fp]),
+    "vhap_grad_clip": (c_i, [c_i, c_fp, c_fp, c_fp, c_fp, c_i, c_f, c_fp, c_sz, c_fp, c_fp]),
+    "vhap_adam_step_clipped": (c_i, [c_i] + [c_fp] * 8 + [c_f] * 4 + [c_fp, c_sz, c_fp, c_i, c_fp]),
     "vhap_set_floats": (c_i, [c_fp, ctypes.POINTER(c_f), c_i, c_fp]),
     "vhap_raster_bin_vnormal": (c_i, [c_fp, c_fp, c_fp] + [c_i] * 5 + [c_fp, c_sz, c_sz, c_i] + [c_fp] * 6),
     "vhap_raster_bin_vnormal_prefill": (c_i, [c_fp, c_fp, c_fp] + [c_i] * 5 + [c_fp, c_sz, c_sz, c_i] + [c_fp] * 5 + [c_fp, c_fp, c_fp, c_i] + [c_fp] * 5),
@@ -135,6 +140,13 @@ SIGNATURES = {
     "vhap_nhwc_maxpool2": (c_i, [c_fp] + [c_i] * 4 + [c_fp, c_fp]),
     "vhap_nhwc_l2norm": (c_i, [c_fp, ctypes.c_longlong, c_i, c_fp, ctypes.c_float, c_fp, c_fp]),
     "vhap_nhwc_add": (c_i, [c_fp, c_fp, c_fp, ctypes.c_longlong, c_fp, c_fp]),
+    "vhap_mx4_quantize": (c_i, [c_fp, c_i, c_ll, c_ll, c_i] + [c_fp] * 3),
+    "vhap_mx4_dequantize": (c_i, [c_fp, c_fp, c_ll, c_i, c_fp, c_i, c_fp]),
+    "vhap_mx4_linear": (c_i, [c_fp, c_i, c_ll, c_ll, c_fp, c_fp, c_ll, c_i] + [c_fp] * 3),
+    "vhap_mx4_linear_input_grad_workspace_bytes": (c_sz, [c_ll, c_ll, c_i]),
+    "vhap_mx4_linear_input_grad": (c_i, [c_fp, c_i, c_ll, c_ll, c_fp, c_fp, c_ll, c_i, c_fp, c_sz, c_fp, c_i, c_fp]),
+    "vhap_mx4_column_sums": (c_i, [c_fp, c_i, c_ll, c_ll, c_ll, c_fp, c_fp]),
+    "vhap_mx4_matmul": (c_i, [c_fp, c_fp, c_ll, c_fp, c_fp, c_ll, c_i, c_fp, c_fp, c_i, c_i, c_fp]),
     "vhap_plan_from_graph": (c_i, [c_fp, c_i, ctypes.POINTER(ctypes.c_void_p)]),
     "vhap_plan_destroy": (c_i, [c_fp]),
     "vhap_plan_set_side_base": (c_i, [c_i]),
@@ -160,6 +172,8 @@ CALL_PLAN_DEFER_JOIN = 64
 CALL_DELTA_UNSCALED = 128
 CALL_TEX_TERMS_CONSUME = 256
 CALL_SKIP_BG_GRAD = 512
+CALL_MX_ACCUMULATE = 1024
+E_NULLPTR, E_BADDIM, E_WORKSPACE, E_HIP, E_UNSUPPORTED = -1, -2, -3, -4, -5
 CONV_IN_RELU, CONV_OUT_RELU, CONV_ACCUMULATE = 1, 2, 4
 
 _lib = None

@@ -1,0 +1,411 @@
+// Global norm over a list of gradients, the gradients scaled to a largest norm, and the Adam update that takes its scale factor from the device.
+//
+//   n = (sum_i sum_j |g_ij|^p)^(1/p), p = 1 or 2;  n = max |g_ij| for p = infinity (a NaN anywhere makes n NaN)
+//   c = min(1, max_norm / (n + 1e-6)), NaN where n is NaN;   out = round(g c)   or   Adam on round32(g c)
+//
+// HBM-bound: the list is read once for n and once for out (the second time from the cache in front of HBM up to some 100 MB), written once.
+// The list is cut into units of 512 elements that never cross a tensor; a WAVE owns a contiguous run of units, so one launch serves tensors of
+// any sizes side by side (one block per tensor or per 4096 elements would leave most lanes of a tracker's ten small tensors idle).  512 blocks
+// of 16 waves fill the chip and leave 512 partial sums: every block of the second launch adds those up itself, in the same order (4 KB out of L2), so
+// there is no third launch, no counter and no atomic -- the same call gives the same bits.
+// The sums are held in 64 bits: the square of an fp32 number is exact there, and no finite gradient overflows.  n is rounded to fp32 once; c is formed
+// from the 64-bit n and rounded to fp32 once.
+// Lists of at most ONE_BLOCK_UNITS units are one block's work in ONE launch (norm, barrier, scale): what counts there is the launches.
+// Measurements: see the bottom of this comment's table in the entry points.
+#include "common.h"
+#include "elem8.h"
+
+#include <algorithm>
+#include <vector>
+
+namespace {
+
+constexpr int GN_T = 1024, GN_WAVES = GN_T / 64, GN_BLOCKS = 512, GN_UNIT = 512;
+constexpr int GN_MAX = 128;                 // tensors per launch: the table travels as kernel arguments (under 4 KB), so a capture keeps it by value
+constexpr long long GN_MOST = 1ll << 39;    // elements of a list: its units are counted in 32 bits
+constexpr int ONE_BLOCK_UNITS = 64;
+
+template <int MAX>
+struct GnTableOf {
+    const void* src[MAX];
+    void* dst[MAX];                         // norm only: unused
+    long long n[MAX];
+    unsigned start[MAX + 1];                // first unit of tensor k
+    unsigned char dtype[MAX];
+    int count;
+};
+using GnTable = GnTableOf<GN_MAX>;
+using GnAdamTable = GnTableOf<VHAP_ADAM_MAX_TENSORS>;
+
+// KIND: 0 = infinity, 1, 2.  An accumulator is a double; for the maximum it holds the BITS of |g| as an integer value: bits order like the numbers they
+// stand for and a NaN lies above infinity, so that it wins the maximum.
+template <int KIND>
+__device__ __forceinline__ double gn_join(double a, double b) { return KIND == 0 ? (a > b ? a : b) : a + b; }
+template <int KIND>
+__device__ __forceinline__ double gn_take(double a, float x) {
+    if constexpr (KIND == 0) return gn_join<0>(a, (double)(__float_as_uint(x) & 0x7fffffffu));
+    if constexpr (KIND == 1) return a + (double)fabsf(x);
+    return fma((double)x, (double)x, a);
+}
+
+// sum (or maximum) over the block, in every thread; the waves are joined in order
+template <int KIND>
+__device__ __forceinline__ double gn_block_join(double v, double* lds) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = gn_join<KIND>(v, __shfl_xor(v, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = lds[0];
+    for (int w = 1; w < (int)(blockDim.x >> 6); w++) s = gn_join<KIND>(s, lds[w]);
+    return s;
+}
+
+template <typename Table>
+__device__ __forceinline__ int gn_find(const Table& t, unsigned unit) {       // the tensor that owns `unit`
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.start[mid] <= unit) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// this wave's run of units, f(tensor, first element of this lane's eight, how many of them exist)
+template <typename Table, typename F>
+__device__ __forceinline__ void gn_units(const Table& t, unsigned wave, unsigned nwaves, F f) {
+    const unsigned units = t.start[t.count];
+    unsigned u = (unsigned)((unsigned long long)units * wave / nwaves);
+    const unsigned u1 = (unsigned)((unsigned long long)units * (wave + 1) / nwaves);
+    if (u >= u1) return;
+    int k = gn_find(t, u);
+    for (; u < u1; u++) {
+        while (u >= t.start[k + 1]) k++;
+        const long long i = (long long)(u - t.start[k]) * GN_UNIT + (threadIdx.x & 63) * 8;
+        const long long left = t.n[k] - i;
+        if (left > 0) f(k, i, left < 8 ? (int)left : 8);
+    }
+}
+
+template <int KIND, typename Table>
+__device__ __forceinline__ double gn_wave_part(const Table& t, unsigned wave, unsigned nwaves) {
+    double a0 = 0., a1 = 0.;
+    gn_units(t, wave, nwaves, [&](int k, long long i, int valid) {
+        float v[8];
+        vhap_load8(t.src[k], i, t.dtype[k], valid, v);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) { a0 = gn_take<KIND>(a0, v[e]); a1 = gn_take<KIND>(a1, v[e + 1]); }
+    });
+    return gn_join<KIND>(a0, a1);
+}
+
+template <int KIND>
+__device__ __forceinline__ double gn_norm_of(double s) {
+    if constexpr (KIND == 0) return (double)__uint_as_float((unsigned)s);
+    if constexpr (KIND == 1) return s;
+    return sqrt(s);
+}
+
+__device__ __forceinline__ float gn_coefficient(double norm, double max_norm) {
+    const double c = max_norm / (norm + 1e-6);
+    return c > 1.0 ? 1.0f : (float)c;                  // (a NaN is not above 1: it stays)
+}
+
+// the partial sums of an earlier launch -> the norm, in every thread
+template <int KIND>
+__device__ __forceinline__ double gn_total(const double* __restrict__ part, int n_part, double* lds) {
+    double s = 0.;
+    for (int i = threadIdx.x; i < n_part; i += blockDim.x) s = gn_join<KIND>(s, part[i]);
+    return gn_norm_of<KIND>(gn_block_join<KIND>(s, lds));
+}
+
+template <int KIND, typename Table>
+__global__ __launch_bounds__(GN_T) void gn_part_kernel(const Table t, double* __restrict__ part, int* step) {
+    __shared__ double lds[GN_WAVES];
+    const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * GN_WAVES + (threadIdx.x >> 6));
+    const double s = gn_block_join<KIND>(gn_wave_part<KIND>(t, wave, gridDim.x * GN_WAVES), lds);
+    if (threadIdx.x == 0) {
+        part[blockIdx.x] = s;
+        if (step && blockIdx.x == 0) step[0] += 1;    // (the Adam launch behind this one reads it)
+    }
+}
+
+template <int KIND>
+__global__ __launch_bounds__(GN_T) void gn_norm_kernel(const double* __restrict__ part, int n_part, float* __restrict__ norm) {
+    __shared__ double lds[GN_WAVES];
+    const double n = gn_total<KIND>(part, n_part, lds);
+    if (threadIdx.x == 0) norm[0] = (float)n;
+}
+
+// part == nullptr: this block is the only one and forms the norm itself
+template <int KIND>
+__global__ __launch_bounds__(GN_T) void gn_scale_kernel(const GnTable t, const double* __restrict__ part, int n_part, double max_norm, float* __restrict__ norm) {
+    __shared__ double lds[GN_WAVES];
+    const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * GN_WAVES + (threadIdx.x >> 6));
+    const double n = part ? gn_total<KIND>(part, n_part, lds) : gn_norm_of<KIND>(gn_block_join<KIND>(gn_wave_part<KIND>(t, wave, GN_WAVES), lds));
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)n;
+    const float c = gn_coefficient(n, max_norm);
+    gn_units(t, wave, gridDim.x * GN_WAVES, [&](int k, long long i, int valid) {
+        if (c == 1.0f && t.src[k] == t.dst[k]) return;                    // in place and not clipped: every element keeps its value
+        float v[8];
+        vhap_load8(t.src[k], i, t.dtype[k], valid, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= c;
+        vhap_store8(t.dst[k], i, t.dtype[k], valid, v);
+    });
+}
+
+struct GnAdam {
+    float* p[VHAP_ADAM_MAX_TENSORS];
+    float* m[VHAP_ADAM_MAX_TENSORS];
+    float* v[VHAP_ADAM_MAX_TENSORS];
+    int lr_index[VHAP_ADAM_MAX_TENSORS];
+};
+
+__device__ __forceinline__ float gn_mul(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;                            // rounded to fp32 before anything is added to it
+}
+
+// vhap_adam_step's update (torch.optim.Adam's arithmetic) on round32(g c).  `step` already counts this step, or (step_add = 1) does not yet.
+__global__ __launch_bounds__(GN_T) void gn_adam_kernel(const GnAdamTable t, const GnAdam a, const double* __restrict__ part, int n_part, double max_norm,
+                                                       float* __restrict__ norm, const float* __restrict__ lr, int* step, int step_add, int bump, float beta1,
+                                                       float beta2, float eps) {
+    __shared__ double lds[GN_WAVES];
+    const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * GN_WAVES + (threadIdx.x >> 6));
+    const float st = (float)(step[0] + step_add);
+    const double n = part ? gn_total<2>(part, n_part, lds) : gn_norm_of<2>(gn_block_join<2>(gn_wave_part<2>(t, wave, GN_WAVES), lds));
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)n;
+    if (bump && threadIdx.x == 0) step[0] += 1;          // (one block; its threads have all read the counter: the join above is a barrier)
+    const float c = gn_coefficient(n, max_norm);
+    const float bc1 = 1.0f - powf(beta1, st), bc2s = sqrtf(1.0f - powf(beta2, st));
+    gn_units(t, wave, gridDim.x * GN_WAVES, [&](int k, long long i, int valid) {
+        const float step_size = lr[a.lr_index[k]] / bc1;
+        float g[8], p[8], m[8], v[8];
+        vhap_load8(t.src[k], i, VHAP_DTYPE_F32, valid, g);
+        vhap_load8(a.p[k], i, VHAP_DTYPE_F32, valid, p);
+        vhap_load8(a.m[k], i, VHAP_DTYPE_F32, valid, m);
+        vhap_load8(a.v[k], i, VHAP_DTYPE_F32, valid, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float gi = gn_mul(g[e], c);         // the clipped gradient as clipping in place would have stored it
+            m[e] = m[e] + (gi - m[e]) * (1.0f - beta1);
+            v[e] = beta2 * v[e] + (1.0f - beta2) * gi * gi;
+            p[e] -= step_size * m[e] / (sqrtf(v[e]) / bc2s + eps);
+        }
+        vhap_store8(a.m[k], i, VHAP_DTYPE_F32, valid, m);
+        vhap_store8(a.v[k], i, VHAP_DTYPE_F32, valid, v);
+        vhap_store8(a.p[k], i, VHAP_DTYPE_F32, valid, p);
+    });
+}
+
+// ---- host side ----
+inline long long gn_units_of(long long n) { return (n + GN_UNIT - 1) / GN_UNIT; }
+
+// Walks the list in launches of at most MAX entries, f(table, units); entries that lie one behind another in memory (views of one flat buffer, source
+// and destination alike) are one entry.
+template <int MAX, typename F>
+int gn_walk(int n_tensors, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, bool merge, F f) {
+    GnTableOf<MAX> t;
+    t.count = 0;
+    unsigned units = 0;
+    for (int k = 0; k < n_tensors; k++) {
+        if (numel[k] == 0) continue;
+        const int dt = dtype ? dtype[k] : VHAP_DTYPE_F32, size = dt == VHAP_DTYPE_F32 ? 4 : 2;
+        if (merge && t.count > 0) {
+            const int j = t.count - 1;
+            const long long was = t.n[j] * size;
+            if (t.dtype[j] == dt && static_cast<const char*>(t.src[j]) + was == src[k] && (!dst || static_cast<char*>(t.dst[j]) + was == dst[k])) {
+                t.n[j] += numel[k];
+                units = t.start[j] + (unsigned)gn_units_of(t.n[j]);
+                continue;
+            }
+        }
+        if (t.count == MAX) {
+            t.start[MAX] = units;
+            const int rc = f(t, units);
+            if (rc != VHAP_OK) return rc;
+            t.count = 0;
+            units = 0;
+        }
+        const int j = t.count++;
+        t.src[j] = src[k];
+        t.dst[j] = dst ? dst[k] : nullptr;
+        t.n[j] = numel[k];
+        t.dtype[j] = (unsigned char)dt;
+        t.start[j] = units;
+        units += (unsigned)gn_units_of(numel[k]);
+    }
+    if (t.count == 0) return VHAP_OK;
+    t.start[t.count] = units;
+    return f(t, units);
+}
+
+int gn_check(int n_tensors, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype) {
+    if (n_tensors < 0) return VHAP_E_BADDIM;
+    if (n_tensors > 0 && (!src || !numel)) return VHAP_E_NULLPTR;
+    long long total = 0;
+    for (int k = 0; k < n_tensors; k++) {
+        if (numel[k] < 0 || numel[k] >= GN_MOST || (dtype && (dtype[k] < 0 || dtype[k] > 2))) return VHAP_E_BADDIM;
+        if (numel[k] > 0 && (!src[k] || (dst && !dst[k]))) return VHAP_E_NULLPTR;
+        total += numel[k];
+        if (total >= GN_MOST) return VHAP_E_BADDIM;
+    }
+    return VHAP_OK;
+}
+
+// What is written must be written once and not be another tensor's input: every destination disjoint from every other destination, and from every
+// source but its own (which it either is, or does not touch).
+struct GnRange {
+    uintptr_t lo, hi;
+    int id;                                  // entry; destinations and sources of an in-place entry carry the same one
+    bool written;
+};
+int gn_disjoint(int n_tensors, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype) {
+    std::vector<GnRange> r;
+    try {
+        int id = 0;
+        gn_walk<GN_MAX>(n_tensors, src, dst, numel, dtype, true, [&](const GnTable& t, unsigned) {
+            for (int k = 0; k < t.count; k++, id++) {
+                const uintptr_t bytes = (uintptr_t)t.n[k] * (t.dtype[k] == VHAP_DTYPE_F32 ? 4 : 2), s = (uintptr_t)t.src[k], d = (uintptr_t)t.dst[k];
+                r.push_back({d, d + bytes, id, true});
+                if (s != d) r.push_back({s, s + bytes, id, false});
+            }
+            return VHAP_OK;
+        });
+        std::sort(r.begin(), r.end(), [](const GnRange& a, const GnRange& b) { return a.lo < b.lo; });
+    } catch (...) {
+        return VHAP_E_HIP;
+    }
+    uintptr_t any = 0, written = 0;          // ends of the furthest range, and of the furthest written one, so far
+    for (const GnRange& x : r) {
+        if (x.lo < written || (x.written && x.lo < any)) return VHAP_E_UNSUPPORTED;
+        any = std::max(any, x.hi);
+        if (x.written) written = std::max(written, x.hi);
+    }
+    return VHAP_OK;
+}
+
+inline int gn_blocks(unsigned units) { return units < (unsigned)GN_BLOCKS * GN_WAVES ? (int)((units + GN_WAVES - 1) / GN_WAVES) : GN_BLOCKS; }
+
+template <int KIND>
+int gn_run(int n_tensors, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, double max_norm, double* part,
+           size_t bytes, float* norm, hipStream_t st) {
+    // how many launches, how many units: one launch of few units is one block's work
+    int launches = 0, n_part = 0;
+    unsigned last = 0;
+    gn_walk<GN_MAX>(n_tensors, src, dst, numel, dtype, true, [&](const GnTable&, unsigned units) {
+        launches++;
+        n_part += gn_blocks(units);
+        last = units;
+        return VHAP_OK;
+    });
+    if (dst && launches == 1 && last <= ONE_BLOCK_UNITS)
+        return gn_walk<GN_MAX>(n_tensors, src, dst, numel, dtype, true, [&](const GnTable& t, unsigned) {
+            gn_scale_kernel<KIND><<<1, GN_T, 0, st>>>(t, nullptr, 0, max_norm, norm);
+            VHAP_LAUNCH_CHECK();
+            return VHAP_OK;
+        });
+    if (n_part > 0 && (!part || bytes < (size_t)n_part * sizeof(double))) return VHAP_E_WORKSPACE;
+    int at = 0;
+    int rc = gn_walk<GN_MAX>(n_tensors, src, dst, numel, dtype, true, [&](const GnTable& t, unsigned units) {
+        const int g = gn_blocks(units);
+        gn_part_kernel<KIND><<<g, GN_T, 0, st>>>(t, part + at, nullptr);
+        at += g;
+        VHAP_LAUNCH_CHECK();
+        return VHAP_OK;
+    });
+    if (rc != VHAP_OK) return rc;
+    if (!dst || launches == 0) {
+        gn_norm_kernel<KIND><<<1, GN_T, 0, st>>>(part, n_part, norm);
+        VHAP_LAUNCH_CHECK();
+        return VHAP_OK;
+    }
+    return gn_walk<GN_MAX>(n_tensors, src, dst, numel, dtype, true, [&](const GnTable& t, unsigned units) {
+        gn_scale_kernel<KIND><<<gn_blocks(units), GN_T, 0, st>>>(t, part, n_part, max_norm, norm);
+        VHAP_LAUNCH_CHECK();
+        return VHAP_OK;
+    });
+}
+
+int gn_dispatch(int norm_kind, int n_tensors, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, double max_norm,
+                void* workspace, size_t bytes, float* norm, hipStream_t st) {
+    double* part = static_cast<double*>(workspace);
+    switch (norm_kind) {
+        case VHAP_NORM_INF: return gn_run<0>(n_tensors, src, dst, numel, dtype, max_norm, part, bytes, norm, st);
+        case 1: return gn_run<1>(n_tensors, src, dst, numel, dtype, max_norm, part, bytes, norm, st);
+        case 2: return gn_run<2>(n_tensors, src, dst, numel, dtype, max_norm, part, bytes, norm, st);
+        default: return VHAP_E_UNSUPPORTED;
+    }
+}
+
+}  // namespace
+
+extern "C" size_t vhap_grad_norm_workspace_bytes(int n_tensors) {
+    return sizeof(double) * GN_BLOCKS * (size_t)(n_tensors <= 0 ? 1 : (n_tensors + GN_MAX - 1) / GN_MAX);      // GN_BLOCKS partial sums a launch at most
+}
+
+extern "C" int vhap_grad_norm(int n_tensors, const void* const* grads, const int64_t* numel, const int32_t* dtype, int norm_kind, void* workspace,
+                              size_t workspace_bytes, float* norm, vhap_stream_t stream) {
+    VHAP_ENTER();
+    if (!norm) return VHAP_E_NULLPTR;
+    const int rc = gn_check(n_tensors, grads, nullptr, numel, dtype);
+    if (rc != VHAP_OK) return rc;
+    return gn_dispatch(norm_kind, n_tensors, grads, nullptr, numel, dtype, 0., workspace, workspace_bytes, norm, vhap_stream(stream));
+}
+
+extern "C" int vhap_grad_clip(int n_tensors, const void* const* grads, void* const* out, const int64_t* numel, const int32_t* dtype, int norm_kind,
+                              float max_norm, void* workspace, size_t workspace_bytes, float* norm, vhap_stream_t stream) {
+    VHAP_ENTER();
+    if (!norm || (n_tensors > 0 && !out)) return VHAP_E_NULLPTR;
+    if (!(max_norm >= 0.f)) return VHAP_E_BADDIM;
+    int rc = gn_check(n_tensors, grads, out, numel, dtype);
+    if (rc == VHAP_OK && n_tensors > 0) rc = gn_disjoint(n_tensors, grads, out, numel, dtype);
+    if (rc != VHAP_OK) return rc;
+    return gn_dispatch(norm_kind, n_tensors, grads, out, numel, dtype, (double)max_norm, workspace, workspace_bytes, norm, vhap_stream(stream));
+}
+
+extern "C" int vhap_adam_step_clipped(int n_tensors, float* const* params, const float* const* grads, float* const* exp_avg, float* const* exp_avg_sq,
+                                      const int64_t* numel, const int32_t* lr_index, const float* lr_device, int32_t* step_device, float beta1,
+                                      float beta2, float eps, float max_norm, void* workspace, size_t workspace_bytes, float* norm, int call_flags,
+                                      vhap_stream_t stream) {
+    VHAP_ENTER();
+    if (!params || !grads || !exp_avg || !exp_avg_sq || !numel || !lr_index || !lr_device || !step_device) return VHAP_E_NULLPTR;
+    if (n_tensors <= 0 || n_tensors > VHAP_ADAM_MAX_TENSORS || !(max_norm >= 0.f)) return VHAP_E_BADDIM;
+    const void* const* src = reinterpret_cast<const void* const*>(grads);
+    const int rc = gn_check(n_tensors, src, nullptr, numel, nullptr);
+    if (rc != VHAP_OK) return rc;
+    GnAdam a{};
+    int n = 0;
+    for (int k = 0; k < n_tensors; k++) {
+        if (numel[k] == 0) continue;              // (gn_walk leaves empty tensors out: the tables stay in step)
+        if (!params[k] || !exp_avg[k] || !exp_avg_sq[k]) return VHAP_E_NULLPTR;
+        if (lr_index[k] < 0) return VHAP_E_BADDIM;
+        a.p[n] = params[k]; a.m[n] = exp_avg[k]; a.v[n] = exp_avg_sq[k]; a.lr_index[n] = lr_index[k];
+        n++;
+    }
+    hipStream_t st = vhap_stream(stream);
+    const bool advanced = (call_flags & VHAP_CALL_ADAM_STEP_ADVANCED) != 0, bump = !advanced && !(call_flags & VHAP_CALL_ADAM_KEEP_STEP);
+    double* part = static_cast<double*>(workspace);
+    if (n == 0) {                                  // nothing but empty tensors: the norm is 0, the step is counted
+        if (norm) {
+            gn_norm_kernel<2><<<1, GN_T, 0, st>>>(part, 0, norm);
+            VHAP_LAUNCH_CHECK();
+        }
+        return bump ? vhap_adam_advance(step_device, stream) : VHAP_OK;
+    }
+    return gn_walk<VHAP_ADAM_MAX_TENSORS>(n_tensors, src, nullptr, numel, nullptr, false, [&](const GnAdamTable& t, unsigned units) {
+        if (units <= ONE_BLOCK_UNITS) {
+            gn_adam_kernel<<<1, GN_T, 0, st>>>(t, a, nullptr, 0, (double)max_norm, norm, lr_device, step_device, advanced ? 0 : 1, bump ? 1 : 0, beta1, beta2, eps);
+            VHAP_LAUNCH_CHECK();
+            return VHAP_OK;
+        }
+        const int g = gn_blocks(units);
+        if (!part || workspace_bytes < (size_t)g * sizeof(double)) return VHAP_E_WORKSPACE;
+        gn_part_kernel<2><<<g, GN_T, 0, st>>>(t, part, bump ? step_device : nullptr);      // (counts the step, unless the caller does)
+        VHAP_LAUNCH_CHECK();
+        gn_adam_kernel<<<g, GN_T, 0, st>>>(t, a, part, g, (double)max_norm, norm, lr_device, step_device, advanced || bump ? 0 : 1, 0, beta1, beta2, eps);
+        VHAP_LAUNCH_CHECK();
+        return VHAP_OK;
+    });
+}

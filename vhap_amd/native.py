@@ -8,9 +8,13 @@ Together they replace the several hundred tiny eager launches per step that the 
     landmark_energy  vertices2landmarks (lbs.py:60-98) + compute_lmk_energy (tracker.py:347-389)
     offset_reg       reg_offset_lap / reg_offset / reg_offset_rigid (tracker.py:552-600)
     tex_prep         get_albedo (tracker.py:247-258) + reg_tex_tv / reg_tex_res_clusters (tracker.py:518-541)
-    HipAdam          torch.optim.Adam (tracker.py:159-211)
+    HipAdam          torch.optim.Adam (tracker.py:159-211), optionally on gradients clipped to a largest global norm
+    grad_norm, clip_by_global_norm, clip_grad_norm_
+                     the norm over a list of gradients and the list scaled to a largest one (vhap_amd/csrc/gradnorm.hip)
 """
+import contextlib
 import ctypes
+import math
 import os
 
 import numpy as np
@@ -374,13 +378,169 @@ def tex_prep(painted, extra, res_mask_u8, w_tv, w_res, scales=None):
 
 
 # ------------------------------------------------------------------------------------------------
+# ---- the global norm over many gradients, and clipping ----
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # VHAP_DTYPE_*
+_NORM_KIND = {1.0: 1, 2.0: 2, math.inf: 0}                                   # VHAP_NORM_INF = 0
+
+
+def on_device(t):
+    """context in which the current device (and so the current stream) is that of tensor `t`"""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _dense(t):
+    """the elements of `t` fill one stretch of memory, each place once (in any order of the axes)"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _grad_list(tensors, what):
+    ts = [tensors] if torch.is_tensor(tensors) else list(tensors)
+    for t in ts:
+        if not torch.is_tensor(t):
+            raise TypeError(f"{what}: expected tensors, got {type(t).__name__}")
+        if t.layout != torch.strided or t.dtype not in _DTYPE_CODE:
+            raise TypeError(f"{what}: dense float32, bfloat16 or float16 tensors, got {t.dtype} ({t.layout})")
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: tensors on a HIP device (no CPU fallback)")
+        if t.device != ts[0].device:
+            raise ValueError(f"{what}: tensors on one device, got {ts[0].device} and {t.device}")
+    return ts
+
+
+def _norm_kind(norm_type):
+    kind = _NORM_KIND.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"norm_type 1, 2 or infinity, got {norm_type}")
+    return kind
+
+
+def _max_norm(v):
+    v = float(v)
+    if not v >= 0.0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {v}")
+    return v
+
+
+def _clip_call(srcs, dsts, kind, max_norm):
+    """vhap_grad_norm (dsts None) / vhap_grad_clip over dense tensors of one device -> the norm, a 0-dim float32 tensor"""
+    L, n, dev = _lib.lib(), len(srcs), srcs[0].device
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    nbytes = L.vhap_grad_norm_workspace_bytes(n)
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev)           # (a workspace of this call's own: calls on other streams, captured ones too, have theirs)
+    if _lib.ACCESS is not None:
+        for t in srcs + (dsts or []):
+            _lib.ACCESS.touch(t)
+    src = (ctypes.c_void_p * n)(*[t.data_ptr() for t in srcs])
+    numel = (ctypes.c_int64 * n)(*[t.numel() for t in srcs])
+    codes = (ctypes.c_int32 * n)(*[_DTYPE_CODE[t.dtype] for t in srcs])
+    with on_device(norm):
+        if dsts is None:
+            _chk(L.vhap_grad_norm(n, src, numel, codes, kind, _p(ws), nbytes, _p(norm), _stream()), "vhap_grad_norm")
+        else:
+            dst = src if dsts is srcs else (ctypes.c_void_p * n)(*[t.data_ptr() for t in dsts])
+            rc = L.vhap_grad_clip(n, src, dst, numel, codes, kind, max_norm, _p(ws), nbytes, _p(norm), _stream())
+            if rc == _lib.E_UNSUPPORTED:
+                raise ValueError("clipping: a result overlaps another result, or another gradient, in memory (the same tensor twice in the list?)")
+            _chk(rc, "vhap_grad_clip")
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(tensors, norm_type=2.0):
+    """The norm over all elements of a list of tensors (float32, bfloat16, float16 side by side; any strides; empty ones count nothing), as a 0-dim
+    float32 tensor on their device: 1-, 2- or infinity-norm, summed in 64 bits in a fixed order.  No synchronisation."""
+    kind, ts = _norm_kind(norm_type), _grad_list(tensors, "grad_norm")
+    if not ts:
+        return torch.zeros(())
+    return _clip_call([t if _dense(t) else t.contiguous() for t in ts], None, kind, 0.0)
+
+
+@torch.no_grad()
+def clip_by_global_norm(grads, max_norm, norm_type=2.0, out=None):
+    """-> (clipped, norm): clipped[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), rounded to its type once; norm as grad_norm.  A NaN norm makes every
+    result NaN.  `out`: tensors like the gradients to write into -- the gradients themselves (in place: a list that is within the limit is then
+    left alone), or memory that overlaps none of them; None: new tensors.  No synchronisation."""
+    kind, max_norm, gs = _norm_kind(norm_type), _max_norm(max_norm), _grad_list(grads, "clip_by_global_norm")
+    if out is None:
+        outs = [torch.empty_like(g, memory_format=torch.contiguous_format) for g in gs]
+    else:
+        outs = _grad_list(out, "clip_by_global_norm(out=)")
+        if len(outs) != len(gs):
+            raise ValueError(f"clip_by_global_norm: {len(gs)} gradients, {len(outs)} results")
+        for g, o in zip(gs, outs):
+            if o.shape != g.shape or o.dtype != g.dtype or o.device != g.device:
+                raise ValueError(f"clip_by_global_norm: a result is like its gradient: {tuple(g.shape)} {g.dtype} {g.device}, got {tuple(o.shape)} {o.dtype} {o.device}")
+    seen = set()
+    for o in outs:
+        if any(st == 0 and n > 1 for st, n in zip(o.stride(), o.shape)):
+            raise ValueError("clip_by_global_norm: a result whose elements share memory (an expanded tensor)")
+        key = (o.data_ptr(), o.shape, o.stride())
+        if o.numel() and key in seen:
+            raise ValueError("clipping: the same tensor twice in the list")
+        seen.add(key)
+    if not gs:
+        return outs, torch.zeros(())
+    # the kernels walk memory in order: a pair that is dense with the same strides is taken as it stands, anything else goes through a contiguous copy
+    srcs, dsts, back = [], [], []
+    for g, o in zip(gs, outs):
+        same = g.stride() == o.stride() or (g.is_contiguous() and o.is_contiguous())
+        if same and _dense(g):
+            srcs.append(g)
+            dsts.append(o)
+        else:
+            c = g.contiguous() if o.data_ptr() != g.data_ptr() else g.clone(memory_format=torch.contiguous_format)
+            t = torch.empty_like(c)
+            srcs.append(c)
+            dsts.append(t)
+            back.append((o, t))
+    norm = _clip_call(srcs, dsts, kind, max_norm)
+    for o, t in back:
+        o.copy_(t)
+    if out is not None:
+        torch.autograd.graph.increment_version(dsts)     # (written behind autograd's back)
+    return outs, norm
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ on the HIP device: the gradients of `parameters` scaled in place to a global norm of at most max_norm; returns the
+    norm they had, a 0-dim float32 tensor.  Parameters without a gradient are skipped.  `error_if_nonfinite`: raise before anything is scaled where the norm
+    is NaN or infinite (waits for the device: not in a capture)."""
+    max_norm, kind = _max_norm(max_norm), _norm_kind(norm_type)
+    ps = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    gs = [p.grad for p in ps if p.grad is not None]
+    if not gs:
+        return torch.zeros((), device=ps[0].device if ps else None)
+    if error_if_nonfinite:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("clip_grad_norm_(error_if_nonfinite=True) reads the norm on the host: not in a stream capture")
+        n = grad_norm(gs, norm_type)
+        if not math.isfinite(float(n)):
+            raise RuntimeError(f"the gradients' norm of order {norm_type} is {float(n)}: not clipped")
+    return clip_by_global_norm(gs, max_norm, norm_type, out=gs)[1]
+
+
 class HipAdam(torch.optim.Optimizer):
     """torch.optim.Adam(params, lr, betas, eps) with the update of ALL parameter tensors in one launch
     (vhap_adam_step).  Same param_groups / lr-scheduler interface; the learning rates and the step counter live on
-    the device so a captured step sees later changes (call sync_lr() after changing group['lr'] outside a capture)."""
+    the device so a captured step sees later changes (call sync_lr() after changing group['lr'] outside a capture).
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8):
+    `max_grad_norm`: every step updates with the gradients clipped to that global 2-norm over all parameters that have one (clip_grad_norm_, then Adam, in two
+    passes over the gradients instead of three and without rewriting them: .grad stays as the backward left it).  The norm before clipping is
+    `grad_norm`, a 0-dim device tensor that every step overwrites.  Such a step cannot be issued in pieces: the norm needs every gradient."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, max_grad_norm=None):
+        if max_grad_norm is not None:
+            max_grad_norm = _max_norm(max_grad_norm)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps))
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
         self._tab = None
         self._lr_host = None
 
@@ -398,6 +558,9 @@ class HipAdam(torch.optim.Optimizer):
         self._step = torch.zeros(1, dtype=torch.int32, device=dev)
         self._lr_dev = torch.zeros(len(self.param_groups), dtype=torch.float32, device=dev)
         n = len(ps)
+        if self.max_grad_norm is not None:
+            self.grad_norm = torch.zeros((), dtype=torch.float32, device=dev)
+            self._clip_ws = torch.empty(_lib.lib().vhap_grad_norm_workspace_bytes(n) // 8, dtype=torch.float64, device=dev)
         P = ctypes.c_void_p * n
         self._tab = {
             "ps": [p for _, p in ps], "n": n,
@@ -436,7 +599,10 @@ class HipAdam(torch.optim.Optimizer):
 
     def fused_update_args(self, p):
         """(exp_avg, exp_avg_sq, lr pointer, step pointer, beta1, beta2, eps) of parameter `p` for a kernel that applies the Adam update itself
-        (vhap_tex_prep_bwd_adam); the caller must still run step(skip=(p,)) to advance the counter.  None if `p` is not ours."""
+        (vhap_tex_prep_bwd_adam); the caller must still run step(skip=(p,)) to advance the counter.  None if `p` is not ours, or if the update
+        needs the norm of every gradient first (max_grad_norm)."""
+        if self.max_grad_norm is not None:
+            return None
         if self._tab is None:
             self._build()
         for gi, g in enumerate(self.param_groups):
@@ -463,6 +629,8 @@ class HipAdam(torch.optim.Optimizer):
         """`only` / `skip` (tensors): update a subset -- a step may be issued in pieces, e.g. the texture as soon as its gradient is
         complete, on a side stream; every piece but the last passes advance=False so that all of them see the same step count
         (or all pass advanced=True after advance())."""
+        if self.max_grad_norm is not None and (only is not None or skip is not None):
+            raise ValueError("HipAdam(max_grad_norm=): the norm is over all gradients, a step cannot be issued in pieces (only= / skip=)")
         if self._tab is None:
             self._build()
         t = self._tab
@@ -487,6 +655,15 @@ class HipAdam(torch.optim.Optimizer):
         G = P(*[t["ps"][i].grad.data_ptr() for i in sel])
         g0 = self.param_groups[0]
         L = _lib.lib()
+        if self.max_grad_norm is not None:
+            with on_device(self.grad_norm):
+                _chk(L.vhap_adam_step_clipped(n, pick(t["p"], ctypes.c_void_p), G, pick(t["m"], ctypes.c_void_p), pick(t["v"], ctypes.c_void_p),
+                                              pick(t["numel"], ctypes.c_int64), pick(t["lr_index"], ctypes.c_int32), _p(self._lr_dev), _p(self._step),
+                                              float(g0["betas"][0]), float(g0["betas"][1]), float(g0["eps"]), self.max_grad_norm, _p(self._clip_ws),
+                                              self._clip_ws.numel() * 8, _p(self.grad_norm),
+                                              _lib.CALL_ADAM_STEP_ADVANCED if advanced else (0 if advance else _lib.CALL_ADAM_KEEP_STEP), _stream()),
+                     "vhap_adam_step_clipped")
+            return
         _chk(L.vhap_adam_step(n, pick(t["p"], ctypes.c_void_p), G, pick(t["m"], ctypes.c_void_p), pick(t["v"], ctypes.c_void_p),
                               pick(t["numel"], ctypes.c_int64), pick(t["lr_index"], ctypes.c_int32), _p(self._lr_dev),
                               _p(self._step), float(g0["betas"][0]), float(g0["betas"][1]), float(g0["eps"]),
