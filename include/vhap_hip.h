@@ -710,7 +710,8 @@ int vhap_adam_step(int n_tensors, float* const* params, const float* const* grad
  * vhap_grad_clip: out[k] = round(grads[k] * c) to the same dtype; out[k] is grads[k] itself (in place; a list that is not clipped is then not rewritten) or
  *   memory of its own: VHAP_E_UNSUPPORTED where a destination overlaps another destination or another tensor's source.  max_norm >= 0.
  * vhap_adam_step_clipped: vhap_adam_step on round(grads * c), the gradients left as they are, the norm over these n_tensors (2-norm; norm may be NULL):
- *   the counter is advanced by the call's own launches (no third one).  call_flags as vhap_adam_step.
+ *   the counter is advanced by the call's own launches (no third one).  call_flags as vhap_adam_step.  The hyperparameters are 64-bit: 1 - beta and
+ *   1 - beta^step are formed there and rounded to float32 once (vhap_adam_step forms them in float32: its 1 - beta2 is off by 1.3e-5 at beta2 = 0.999).
  * Lists of at most 32768 elements (by units of 512 a tensor) are one launch, others two, and two more for every further 128 tensors that do not lie one
  * behind another in memory. */
 #define VHAP_NORM_INF 0
@@ -721,10 +722,10 @@ size_t vhap_grad_norm_workspace_bytes(int n_tensors);
 int vhap_grad_norm(int n_tensors, const void* const* grads, const int64_t* numel, const int32_t* dtype, int norm_kind,
                    void* workspace, size_t workspace_bytes, float* norm, vhap_stream_t stream);
 int vhap_grad_clip(int n_tensors, const void* const* grads, void* const* out, const int64_t* numel, const int32_t* dtype,
-                   int norm_kind, float max_norm, void* workspace, size_t workspace_bytes, float* norm, vhap_stream_t stream);
+                   int norm_kind, double max_norm, void* workspace, size_t workspace_bytes, float* norm, vhap_stream_t stream);
 int vhap_adam_step_clipped(int n_tensors, float* const* params, const float* const* grads, float* const* exp_avg,
                            float* const* exp_avg_sq, const int64_t* numel, const int32_t* lr_index, const float* lr_device,
-                           int32_t* step_device, float beta1, float beta2, float eps, float max_norm, void* workspace,
+                           int32_t* step_device, double beta1, double beta2, double eps, double max_norm, void* workspace,
                            size_t workspace_bytes, float* norm, int call_flags, vhap_stream_t stream);
 /* step_device[0] += 1 (one tiny launch): advance the counter at the HEAD of a step, then issue the step's vhap_adam_step calls with
  * VHAP_CALL_ADAM_STEP_ADVANCED. */

@@ -17,6 +17,7 @@ c_i = ctypes.c_int
 c_sz = ctypes.c_size_t
 c_f = ctypes.c_float
 c_ll = ctypes.c_longlong
+c_d = ctypes.c_double
 
 # name -> (restype, [argtypes]) ; must list EVERY symbol declared in include/vhap_hip.h
 SIGNATURES = {
@@ -122,8 +123,8 @@ SIGNATURES = {
     "vhap_adam_advance": (c_i, [c_fp, c_fp]),
     "vhap_grad_norm_workspace_bytes": (c_sz, [c_i]),
     "vhap_grad_norm": (c_i, [c_i, c_fp, c_fp, c_fp, c_i, c_fp, c_sz, c_fp, c_fp]),
-    "vhap_grad_clip": (c_i, [c_i, c_fp, c_fp, c_fp, c_fp, c_i, c_f, c_fp, c_sz, c_fp, c_fp]),
-    "vhap_adam_step_clipped": (c_i, [c_i] + [c_fp] * 8 + [c_f] * 4 + [c_fp, c_sz, c_fp, c_i, c_fp]),
+    "vhap_grad_clip": (c_i, [c_i, c_fp, c_fp, c_fp, c_fp, c_i, c_d, c_fp, c_sz, c_fp, c_fp]),
+    "vhap_adam_step_clipped": (c_i, [c_i] + [c_fp] * 8 + [c_d] * 4 + [c_fp, c_sz, c_fp, c_i, c_fp]),
     "vhap_set_floats": (c_i, [c_fp, ctypes.POINTER(c_f), c_i, c_fp]),
     "vhap_raster_bin_vnormal": (c_i, [c_fp, c_fp, c_fp] + [c_i] * 5 + [c_fp, c_sz, c_sz, c_i] + [c_fp] * 6),
     "vhap_raster_bin_vnormal_prefill": (c_i, [c_fp, c_fp, c_fp] + [c_i] * 5 + [c_fp, c_sz, c_sz, c_i] + [c_fp] * 5 + [c_fp, c_fp, c_fp, c_i] + [c_fp] * 5),
@@ -199,6 +200,29 @@ def lib():
             raise VhapHipError("libvhap_hip.so ABI version mismatch")
         _lib = L
     return _lib
+
+
+_host = None
+
+
+def host():
+    """The extension module csrc/host.cpp over this library's entry points (no fallback, like lib()): the calls whose host time would otherwise exceed their
+    kernels'.  It does not report to a recording capture (ACCESS): the nodes of its calls count as unknown there, and such a plan does not defer its join."""
+    global _host
+    if _host is None:
+        import importlib.machinery
+        import importlib.util
+        L = lib()
+        path = os.path.join(_HERE, "lib", "vhap_host.so")
+        if not os.path.exists(path):
+            raise VhapHipError(f"{path} not found: build it with `python -m vhap_amd.build`")
+        loader = importlib.machinery.ExtensionFileLoader("vhap_host", path)
+        m = importlib.util.module_from_spec(importlib.util.spec_from_loader("vhap_host", loader))
+        loader.exec_module(m)
+        names = [n for n in SIGNATURES if n == "vhap_strerror" or n.startswith(("vhap_grad_", "vhap_mx4_"))]
+        m.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names}, VhapHipError)
+        _host = m
+    return _host
 
 
 def debug_set_flags(flags):

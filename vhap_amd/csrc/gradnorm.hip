@@ -167,18 +167,22 @@ __device__ __forceinline__ float gn_mul(float a, float b) {
     return a * b;                            // rounded to fp32 before anything is added to it
 }
 
-// vhap_adam_step's update (torch.optim.Adam's arithmetic) on round32(g c).  `step` already counts this step, or (step_add = 1) does not yet.
+// torch.optim.Adam's update on round32(g c).  `step` already counts this step, or (step_add = 1) does not yet.
 __global__ __launch_bounds__(GN_T) void gn_adam_kernel(const GnAdamTable t, const GnAdam a, const double* __restrict__ part, int n_part, double max_norm,
-                                                       float* __restrict__ norm, const float* __restrict__ lr, int* step, int step_add, int bump, float beta1,
-                                                       float beta2, float eps) {
+                                                       float* __restrict__ norm, const float* __restrict__ lr, int* step, int step_add, int bump, double beta1,
+                                                       double beta2, float eps) {
     __shared__ double lds[GN_WAVES];
+    __shared__ float bias_correction[2];
     const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * GN_WAVES + (threadIdx.x >> 6));
-    const float st = (float)(step[0] + step_add);
+    if (threadIdx.x < 2) {                               // 1 - beta1^t and the root of 1 - beta2^t (read behind the join's barriers)
+        const double left = 1.0 - pow(threadIdx.x ? beta2 : beta1, (double)(step[0] + step_add));
+        bias_correction[threadIdx.x] = (float)(threadIdx.x ? sqrt(left) : left);
+    }
     const double n = part ? gn_total<2>(part, n_part, lds) : gn_norm_of<2>(gn_block_join<2>(gn_wave_part<2>(t, wave, GN_WAVES), lds));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)n;
-    if (bump && threadIdx.x == 0) step[0] += 1;          // (one block; its threads have all read the counter: the join above is a barrier)
+    if (bump && threadIdx.x == 0) step[0] += 1;          // (one block; what reads the counter has done so: the join above is a barrier)
     const float c = gn_coefficient(n, max_norm);
-    const float bc1 = 1.0f - powf(beta1, st), bc2s = sqrtf(1.0f - powf(beta2, st));
+    const float bc1 = bias_correction[0], bc2s = bias_correction[1], b2 = (float)beta2, left1 = (float)(1.0 - beta1), left2 = (float)(1.0 - beta2);
     gn_units(t, wave, gridDim.x * GN_WAVES, [&](int k, long long i, int valid) {
         const float step_size = lr[a.lr_index[k]] / bc1;
         float g[8], p[8], m[8], v[8];
@@ -189,8 +193,8 @@ __global__ __launch_bounds__(GN_T) void gn_adam_kernel(const GnAdamTable t, cons
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float gi = gn_mul(g[e], c);         // the clipped gradient as clipping in place would have stored it
-            m[e] = m[e] + (gi - m[e]) * (1.0f - beta1);
-            v[e] = beta2 * v[e] + (1.0f - beta2) * gi * gi;
+            m[e] = m[e] + (gi - m[e]) * left1;
+            v[e] = b2 * v[e] + left2 * gi * gi;
             p[e] -= step_size * m[e] / (sqrtf(v[e]) / bc2s + eps);
         }
         vhap_store8(a.m[k], i, VHAP_DTYPE_F32, valid, m);
@@ -355,23 +359,23 @@ extern "C" int vhap_grad_norm(int n_tensors, const void* const* grads, const int
 }
 
 extern "C" int vhap_grad_clip(int n_tensors, const void* const* grads, void* const* out, const int64_t* numel, const int32_t* dtype, int norm_kind,
-                              float max_norm, void* workspace, size_t workspace_bytes, float* norm, vhap_stream_t stream) {
+                              double max_norm, void* workspace, size_t workspace_bytes, float* norm, vhap_stream_t stream) {
     VHAP_ENTER();
     if (!norm || (n_tensors > 0 && !out)) return VHAP_E_NULLPTR;
-    if (!(max_norm >= 0.f)) return VHAP_E_BADDIM;
+    if (!(max_norm >= 0.)) return VHAP_E_BADDIM;
     int rc = gn_check(n_tensors, grads, out, numel, dtype);
     if (rc == VHAP_OK && n_tensors > 0) rc = gn_disjoint(n_tensors, grads, out, numel, dtype);
     if (rc != VHAP_OK) return rc;
-    return gn_dispatch(norm_kind, n_tensors, grads, out, numel, dtype, (double)max_norm, workspace, workspace_bytes, norm, vhap_stream(stream));
+    return gn_dispatch(norm_kind, n_tensors, grads, out, numel, dtype, max_norm, workspace, workspace_bytes, norm, vhap_stream(stream));
 }
 
 extern "C" int vhap_adam_step_clipped(int n_tensors, float* const* params, const float* const* grads, float* const* exp_avg, float* const* exp_avg_sq,
-                                      const int64_t* numel, const int32_t* lr_index, const float* lr_device, int32_t* step_device, float beta1,
-                                      float beta2, float eps, float max_norm, void* workspace, size_t workspace_bytes, float* norm, int call_flags,
+                                      const int64_t* numel, const int32_t* lr_index, const float* lr_device, int32_t* step_device, double beta1,
+                                      double beta2, double eps, double max_norm, void* workspace, size_t workspace_bytes, float* norm, int call_flags,
                                       vhap_stream_t stream) {
     VHAP_ENTER();
     if (!params || !grads || !exp_avg || !exp_avg_sq || !numel || !lr_index || !lr_device || !step_device) return VHAP_E_NULLPTR;
-    if (n_tensors <= 0 || n_tensors > VHAP_ADAM_MAX_TENSORS || !(max_norm >= 0.f)) return VHAP_E_BADDIM;
+    if (n_tensors <= 0 || n_tensors > VHAP_ADAM_MAX_TENSORS || !(max_norm >= 0.)) return VHAP_E_BADDIM;
     const void* const* src = reinterpret_cast<const void* const*>(grads);
     const int rc = gn_check(n_tensors, src, nullptr, numel, nullptr);
     if (rc != VHAP_OK) return rc;
@@ -396,7 +400,7 @@ extern "C" int vhap_adam_step_clipped(int n_tensors, float* const* params, const
     }
     return gn_walk<VHAP_ADAM_MAX_TENSORS>(n_tensors, src, nullptr, numel, nullptr, false, [&](const GnAdamTable& t, unsigned units) {
         if (units <= ONE_BLOCK_UNITS) {
-            gn_adam_kernel<<<1, GN_T, 0, st>>>(t, a, nullptr, 0, (double)max_norm, norm, lr_device, step_device, advanced ? 0 : 1, bump ? 1 : 0, beta1, beta2, eps);
+            gn_adam_kernel<<<1, GN_T, 0, st>>>(t, a, nullptr, 0, max_norm, norm, lr_device, step_device, advanced ? 0 : 1, bump ? 1 : 0, beta1, beta2, (float)eps);
             VHAP_LAUNCH_CHECK();
             return VHAP_OK;
         }
@@ -404,7 +408,7 @@ extern "C" int vhap_adam_step_clipped(int n_tensors, float* const* params, const
         if (!part || workspace_bytes < (size_t)g * sizeof(double)) return VHAP_E_WORKSPACE;
         gn_part_kernel<2><<<g, GN_T, 0, st>>>(t, part, bump ? step_device : nullptr);      // (counts the step, unless the caller does)
         VHAP_LAUNCH_CHECK();
-        gn_adam_kernel<<<g, GN_T, 0, st>>>(t, a, part, g, (double)max_norm, norm, lr_device, step_device, advanced || bump ? 0 : 1, 0, beta1, beta2, eps);
+        gn_adam_kernel<<<g, GN_T, 0, st>>>(t, a, part, g, max_norm, norm, lr_device, step_device, advanced || bump ? 0 : 1, 0, beta1, beta2, (float)eps);
         VHAP_LAUNCH_CHECK();
         return VHAP_OK;
     });

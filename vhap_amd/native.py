@@ -388,30 +388,8 @@ def on_device(t):
     return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
-def _dense(t):
-    """the elements of `t` fill one stretch of memory, each place once (in any order of the axes)"""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-def _grad_list(tensors, what):
-    ts = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    for t in ts:
-        if not torch.is_tensor(t):
-            raise TypeError(f"{what}: expected tensors, got {type(t).__name__}")
-        if t.layout != torch.strided or t.dtype not in _DTYPE_CODE:
-            raise TypeError(f"{what}: dense float32, bfloat16 or float16 tensors, got {t.dtype} ({t.layout})")
-        if not t.is_cuda:
-            raise RuntimeError(f"{what}: tensors on a HIP device (no CPU fallback)")
-        if t.device != ts[0].device:
-            raise ValueError(f"{what}: tensors on one device, got {ts[0].device} and {t.device}")
-    return ts
+def _tensors(ts):
+    return [ts] if torch.is_tensor(ts) else ts if isinstance(ts, (list, tuple)) else list(ts)
 
 
 def _norm_kind(norm_type):
@@ -428,84 +406,19 @@ def _max_norm(v):
     return v
 
 
-def _clip_call(srcs, dsts, kind, max_norm):
-    """vhap_grad_norm (dsts None) / vhap_grad_clip over dense tensors of one device -> the norm, a 0-dim float32 tensor"""
-    L, n, dev = _lib.lib(), len(srcs), srcs[0].device
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = L.vhap_grad_norm_workspace_bytes(n)
-    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev)           # (a workspace of this call's own: calls on other streams, captured ones too, have theirs)
-    if _lib.ACCESS is not None:
-        for t in srcs + (dsts or []):
-            _lib.ACCESS.touch(t)
-    src = (ctypes.c_void_p * n)(*[t.data_ptr() for t in srcs])
-    numel = (ctypes.c_int64 * n)(*[t.numel() for t in srcs])
-    codes = (ctypes.c_int32 * n)(*[_DTYPE_CODE[t.dtype] for t in srcs])
-    with on_device(norm):
-        if dsts is None:
-            _chk(L.vhap_grad_norm(n, src, numel, codes, kind, _p(ws), nbytes, _p(norm), _stream()), "vhap_grad_norm")
-        else:
-            dst = src if dsts is srcs else (ctypes.c_void_p * n)(*[t.data_ptr() for t in dsts])
-            rc = L.vhap_grad_clip(n, src, dst, numel, codes, kind, max_norm, _p(ws), nbytes, _p(norm), _stream())
-            if rc == _lib.E_UNSUPPORTED:
-                raise ValueError("clipping: a result overlaps another result, or another gradient, in memory (the same tensor twice in the list?)")
-            _chk(rc, "vhap_grad_clip")
-    return norm
-
-
-@torch.no_grad()
 def grad_norm(tensors, norm_type=2.0):
     """The norm over all elements of a list of tensors (float32, bfloat16, float16 side by side; any strides; empty ones count nothing), as a 0-dim
     float32 tensor on their device: 1-, 2- or infinity-norm, summed in 64 bits in a fixed order.  No synchronisation."""
-    kind, ts = _norm_kind(norm_type), _grad_list(tensors, "grad_norm")
-    if not ts:
-        return torch.zeros(())
-    return _clip_call([t if _dense(t) else t.contiguous() for t in ts], None, kind, 0.0)
+    return _lib.host().grad_norm(_tensors(tensors), _norm_kind(norm_type))
 
 
-@torch.no_grad()
 def clip_by_global_norm(grads, max_norm, norm_type=2.0, out=None):
     """-> (clipped, norm): clipped[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), rounded to its type once; norm as grad_norm.  A NaN norm makes every
     result NaN.  `out`: tensors like the gradients to write into -- the gradients themselves (in place: a list that is within the limit is then
     left alone), or memory that overlaps none of them; None: new tensors.  No synchronisation."""
-    kind, max_norm, gs = _norm_kind(norm_type), _max_norm(max_norm), _grad_list(grads, "clip_by_global_norm")
-    if out is None:
-        outs = [torch.empty_like(g, memory_format=torch.contiguous_format) for g in gs]
-    else:
-        outs = _grad_list(out, "clip_by_global_norm(out=)")
-        if len(outs) != len(gs):
-            raise ValueError(f"clip_by_global_norm: {len(gs)} gradients, {len(outs)} results")
-        for g, o in zip(gs, outs):
-            if o.shape != g.shape or o.dtype != g.dtype or o.device != g.device:
-                raise ValueError(f"clip_by_global_norm: a result is like its gradient: {tuple(g.shape)} {g.dtype} {g.device}, got {tuple(o.shape)} {o.dtype} {o.device}")
-    seen = set()
-    for o in outs:
-        if any(st == 0 and n > 1 for st, n in zip(o.stride(), o.shape)):
-            raise ValueError("clip_by_global_norm: a result whose elements share memory (an expanded tensor)")
-        key = (o.data_ptr(), o.shape, o.stride())
-        if o.numel() and key in seen:
-            raise ValueError("clipping: the same tensor twice in the list")
-        seen.add(key)
-    if not gs:
-        return outs, torch.zeros(())
-    # the kernels walk memory in order: a pair that is dense with the same strides is taken as it stands, anything else goes through a contiguous copy
-    srcs, dsts, back = [], [], []
-    for g, o in zip(gs, outs):
-        same = g.stride() == o.stride() or (g.is_contiguous() and o.is_contiguous())
-        if same and _dense(g):
-            srcs.append(g)
-            dsts.append(o)
-        else:
-            c = g.contiguous() if o.data_ptr() != g.data_ptr() else g.clone(memory_format=torch.contiguous_format)
-            t = torch.empty_like(c)
-            srcs.append(c)
-            dsts.append(t)
-            back.append((o, t))
-    norm = _clip_call(srcs, dsts, kind, max_norm)
-    for o, t in back:
-        o.copy_(t)
-    if out is not None:
-        torch.autograd.graph.increment_version(dsts)     # (written behind autograd's back)
-    return outs, norm
+    grads = _tensors(grads)
+    out = grads if out is grads else out if out is None else _tensors(out)
+    return _lib.host().clip(grads, out, _norm_kind(norm_type), _max_norm(max_norm))
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -532,7 +445,8 @@ class HipAdam(torch.optim.Optimizer):
     the device so a captured step sees later changes (call sync_lr() after changing group['lr'] outside a capture).
 
     `max_grad_norm`: every step updates with the gradients clipped to that global 2-norm over all parameters that have one (clip_grad_norm_, then Adam, in two
-    passes over the gradients instead of three and without rewriting them: .grad stays as the backward left it).  The norm before clipping is
+    passes over the gradients instead of three and without rewriting them: .grad stays as the backward left it; 1 - beta2 and the bias corrections are formed in
+    64 bits there, so that the update is nearer to torch's than the unclipped one, which forms them in fp32).  The norm before clipping is
     `grad_norm`, a 0-dim device tensor that every step overwrites.  Such a step cannot be issued in pieces: the norm needs every gradient."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, max_grad_norm=None):
@@ -636,6 +550,8 @@ class HipAdam(torch.optim.Optimizer):
         t = self._tab
         if not torch.cuda.is_current_stream_capturing():
             self.sync_lr()
+        if self.max_grad_norm is not None:
+            return self._step_clipped(advance, advanced)
         pick_p = lambda p: (only is None or any(p is q for q in only)) and (skip is None or not any(p is q for q in skip))
         sel = [i for i, p in enumerate(t["ps"]) if p.grad is not None and pick_p(p)]      # like torch: parameters without .grad are skipped
         if not sel:
@@ -655,17 +571,34 @@ class HipAdam(torch.optim.Optimizer):
         G = P(*[t["ps"][i].grad.data_ptr() for i in sel])
         g0 = self.param_groups[0]
         L = _lib.lib()
-        if self.max_grad_norm is not None:
-            with on_device(self.grad_norm):
-                _chk(L.vhap_adam_step_clipped(n, pick(t["p"], ctypes.c_void_p), G, pick(t["m"], ctypes.c_void_p), pick(t["v"], ctypes.c_void_p),
-                                              pick(t["numel"], ctypes.c_int64), pick(t["lr_index"], ctypes.c_int32), _p(self._lr_dev), _p(self._step),
-                                              float(g0["betas"][0]), float(g0["betas"][1]), float(g0["eps"]), self.max_grad_norm, _p(self._clip_ws),
-                                              self._clip_ws.numel() * 8, _p(self.grad_norm),
-                                              _lib.CALL_ADAM_STEP_ADVANCED if advanced else (0 if advance else _lib.CALL_ADAM_KEEP_STEP), _stream()),
-                     "vhap_adam_step_clipped")
-            return
         _chk(L.vhap_adam_step(n, pick(t["p"], ctypes.c_void_p), G, pick(t["m"], ctypes.c_void_p), pick(t["v"], ctypes.c_void_p),
                               pick(t["numel"], ctypes.c_int64), pick(t["lr_index"], ctypes.c_int32), _p(self._lr_dev),
                               _p(self._step), float(g0["betas"][0]), float(g0["betas"][1]), float(g0["eps"]),
                               _lib.CALL_ADAM_STEP_ADVANCED if advanced else (0 if advance else _lib.CALL_ADAM_KEEP_STEP), _stream()),
              "vhap_adam_step")
+
+    def _step_clipped(self, advance, advanced):
+        t = self._tab
+        ps, grads = t["ps"], [p.grad for p in t["ps"]]
+        sel = tuple(i for i, g in enumerate(grads) if g is not None)
+        if not sel:
+            return
+        for i in sel:
+            if not grads[i].is_contiguous():
+                grads[i] = ps[i].grad = grads[i].contiguous()
+        n = len(sel)
+        tab = t.setdefault("clip", {}).get(sel)       # the pointer tables of what the optimiser itself holds, per set of parameters that have a gradient
+        if tab is None:
+            pick = lambda arr, ty: (ty * n)(*[arr[i] for i in sel])
+            P = ctypes.c_void_p
+            tab = t["clip"][sel] = (pick(t["p"], P), pick(t["m"], P), pick(t["v"], P), pick(t["numel"], ctypes.c_int64), pick(t["lr_index"], ctypes.c_int32), P * n)
+        if _lib.ACCESS is not None:                   # (pointer tables: tell a recording capture what this call touches)
+            for i in sel:
+                for x in (ps[i], grads[i], self.state[ps[i]]["exp_avg"], self.state[ps[i]]["exp_avg_sq"]):
+                    _lib.ACCESS.touch(x)
+        g0 = self.param_groups[0]
+        with on_device(self.grad_norm):
+            _chk(_lib.lib().vhap_adam_step_clipped(n, tab[0], tab[5](*[grads[i].data_ptr() for i in sel]), tab[1], tab[2], tab[3], tab[4], _p(self._lr_dev), _p(self._step),
+                                                   g0["betas"][0], g0["betas"][1], g0["eps"], self.max_grad_norm, _p(self._clip_ws), self._clip_ws.numel() * 8, _p(self.grad_norm),
+                                                   _lib.CALL_ADAM_STEP_ADVANCED if advanced else (0 if advance else _lib.CALL_ADAM_KEEP_STEP), _stream()),
+                 "vhap_adam_step_clipped")
