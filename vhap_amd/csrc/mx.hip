@@ -37,17 +37,24 @@ struct MxMatrix {
 
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float(byte << 23); }   // what the conversions take: they read the exponent field (0: 2^-127, 255: NaN)
 
-// the 16 bytes of codes and the scale byte of block `blk` of `row`; a row or block outside the matrix is zeros with scale 1
+// the 16 bytes of codes and the scale byte of block `blk` of `row`; behind the last row or block: the last one's, without a branch around the load.  Nothing is wrong with that
+// where the other operand is zero behind the last block (or row, in the input's gradient) and results behind the last row are not stored: a product with zero is
+// zero, or NaN where that last block is NaN and the sum is NaN already.
 __device__ __forceinline__ uint4 mx_block(const MxMatrix& w, long long row, int blk, unsigned& scale) {
-    const bool ok = row < w.rows && blk < w.Kb;
-    const size_t at = ok ? (size_t)row * w.Kb + blk : 0;
-    uint4 c = reinterpret_cast<const uint4*>(w.codes)[at];
+    const size_t at = (size_t)min(row, w.rows - 1) * w.Kb + min(blk, w.Kb - 1);
     scale = w.scales[at];
-    if (!ok) {
-        c = uint4{0u, 0u, 0u, 0u};
-        scale = 127u;
-    }
-    return c;
+    return reinterpret_cast<const uint4*>(w.codes)[at];
+}
+
+// The same for a matrix instruction's operand: lane (r, q) = (lane % 16, lane / 16) gets block k + q of row row_of(r).  Read in that order, sixteen neighbouring lanes would
+// touch sixteen rows, four times over; read four lanes a row and passed on across the wave, neighbours read 64 consecutive bytes.
+template <typename F>
+__device__ __forceinline__ uint4 mx_operand(const MxMatrix& w, F row_of, int k, unsigned& scale) {
+    const int lane = threadIdx.x & 63, from = 4 * (4 * (lane & 15) + (lane >> 4));
+    const uint4 c = mx_block(w, row_of(lane >> 2), k + (lane & 3), scale);
+    scale = (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)scale);
+    return uint4{(unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.x), (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.y),
+                 (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.z), (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.w)};
 }
 
 __device__ __forceinline__ unsigned mx_pair_bits(bf16x2 v) { return __builtin_bit_cast(unsigned, v); }
@@ -95,6 +102,51 @@ __device__ __forceinline__ void mx_split8(const float (&v)[8], bf16x8 (&out)[P])
         r.z = t[4][p] >> 16 | t[5][p];
         r.w = t[6][p] >> 16 | t[7][p];
         out[p] = __builtin_bit_cast(bf16x8, r);
+    }
+}
+
+// eight elements as they lie in memory: a load that is to be in flight under other work must not be converted where it is issued
+template <int DT>
+struct MxRaw8 {
+    unsigned w[DT == VHAP_DTYPE_F32 ? 8 : 4];
+};
+template <int DT>
+__device__ __forceinline__ void mx_load_raw8(const void* p, long long i, int valid, MxRaw8<DT>& r) {
+    if constexpr (DT == VHAP_DTYPE_F32) {
+        const float* q = static_cast<const float*>(p) + i;
+        if (valid >= 8) {
+            const VhapVec16a4 a = *reinterpret_cast<const VhapVec16a4*>(q), b = *reinterpret_cast<const VhapVec16a4*>(q + 4);
+#pragma unroll
+            for (int k = 0; k < 4; k++) { r.w[k] = a.w[k]; r.w[4 + k] = b.w[k]; }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) r.w[k] = k < valid ? __float_as_uint(q[k]) : 0u;
+        }
+    } else {
+        const unsigned short* q = static_cast<const unsigned short*>(p) + i;
+        if (valid >= 8) {
+            const VhapVec16a2 a = *reinterpret_cast<const VhapVec16a2*>(q);
+#pragma unroll
+            for (int k = 0; k < 4; k++) r.w[k] = a.w[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) r.w[k] = (2 * k < valid ? (unsigned)q[2 * k] : 0u) | (2 * k + 1 < valid ? (unsigned)q[2 * k + 1] << 16 : 0u);
+        }
+    }
+}
+// their P bf16 fragments (bf16: as they are)
+template <int DT>
+__device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[mx_pieces<DT>()]) {
+    if constexpr (DT == VHAP_DTYPE_BF16) {
+        out[0] = __builtin_bit_cast(bf16x8, r);
+    } else {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if constexpr (DT == VHAP_DTYPE_F32) v[k] = __uint_as_float(r.w[k]);
+            else v[k] = __half2float(__ushort_as_half((unsigned short)(r.w[k >> 1] >> 16 * (k & 1))));
+        }
+        mx_split8<mx_pieces<DT>()>(v, out);
     }
 }
 
@@ -177,6 +229,92 @@ __device__ __forceinline__ void mx_store_row(const MxLinear& a, long long m, lon
     }
 }
 
+template <int DT>
+__device__ __forceinline__ float mx_one(const void* p, long long i) {
+    if constexpr (DT == VHAP_DTYPE_F32) return static_cast<const float*>(p)[i];
+    if constexpr (DT == VHAP_DTYPE_BF16) return __uint_as_float((unsigned)static_cast<const unsigned short*>(p)[i] << 16);
+    return __half2float(static_cast<const __half*>(p)[i]);
+}
+template <int DT>
+__device__ __forceinline__ void mx_put(void* p, long long i, float v) {
+    if constexpr (DT == VHAP_DTYPE_F32) static_cast<float*>(p)[i] = v;
+    if constexpr (DT == VHAP_DTYPE_BF16) static_cast<unsigned short*>(p)[i] = (unsigned short)vhap_bf16_bits(v);
+    if constexpr (DT == VHAP_DTYPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+// the 32 numbers of a block, scaled
+__device__ __forceinline__ void mx_decode32(const uint4& c, float scale, float (&v)[32]) {
+    const unsigned w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+        const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[d], scale, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[d], scale, 1);
+        const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[d], scale, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[d], scale, 3);
+        v[8 * d] = p0.x; v[8 * d + 1] = p0.y; v[8 * d + 2] = p1.x; v[8 * d + 3] = p1.y;
+        v[8 * d + 4] = p2.x; v[8 * d + 5] = p2.y; v[8 * d + 6] = p3.x; v[8 * d + 7] = p3.y;
+    }
+}
+
+// One or two rows of x, K up to 128 KS: four lanes a row of W, a block of 32 each, against their 32 elements of x in registers -- 16 conversions and 32 M multiply-adds
+// for 16 bytes, under what memory delivers, and consecutive lanes read consecutive memory (in the matrix instruction's order they do not: see below).
+template <int DT, int MM, int KS>
+__global__ __launch_bounds__(MX_T) void mx_linear_row_kernel(const MxLinear a) {
+    const int lane = threadIdx.x & 63, b = lane & 3, r = lane >> 2;
+    float x[MM][KS][32];
+#pragma unroll
+    for (int m = 0; m < MM; m++)
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int k0 = 128 * ks + 32 * b + 8 * j;
+                float v[8];
+                vhap_load8(a.x, m * a.ldx + k0, DT, m < a.M ? mx_left(k0, a.w.K) : 0, v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[m][ks][8 * j + e] = v[e];
+            }
+    const long long groups = (a.w.rows + 63) / 64;
+    for (long long g = (long long)blockIdx.x * (MX_T / 64) + (threadIdx.x >> 6); g < groups; g += (long long)gridDim.x * (MX_T / 64)) {
+        uint4 c[4][KS];
+        unsigned s[4][KS];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) c[t][ks] = mx_block(a.w, g * 64 + 16 * t + r, 4 * ks + b, s[t][ks]);
+        const long long n = g * 64 + 16 * b + r;                  // the column that this lane keeps: tile b's
+        const float bias = a.bias && n < a.w.rows ? a.bias[n] : 0.f;
+        float mine[MM];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            float sum[MM];
+#pragma unroll
+            for (int m = 0; m < MM; m++) sum[m] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                float w[32];
+                mx_decode32(c[t][ks], mx_scale(s[t][ks]), w);
+#pragma unroll
+                for (int m = 0; m < MM; m++) {
+                    float p0 = 0.f, p1 = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        p0 = fmaf(w[e], x[m][ks][e], p0);
+                        p1 = fmaf(w[e + 1], x[m][ks][e + 1], p1);
+                    }
+                    sum[m] += p0 + p1;
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MM; m++) {
+                sum[m] += vhap_dpp<0xB1>(sum[m]);                 // quad_perm [1,0,3,2]
+                sum[m] += vhap_dpp<0x4E>(sum[m]);                 // quad_perm [2,3,0,1]
+                mine[m] = t == 0 ? sum[m] : b == t ? sum[m] : mine[m];
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MM; m++)
+            if (m < a.M && n < a.w.rows) mx_put<DT>(a.y, m * a.w.rows + n, a.bias ? mine[m] + bias : mine[m]);
+    }
+}
+
 // Few rows of x (M times its pieces fit the 16 columns of ONE matrix instruction) and K up to 128 KS: the x fragments stay in registers, every wave streams groups of
 // 64 rows of W through them.  Column c holds piece c % P of row c / P; the pieces' sums are joined across neighbouring lanes at the end.
 // Operand rows are dealt out so that a lane ends with 16 CONSECUTIVE columns of y: tile t, row r of the instruction is row 16 (r / 4) + 4 t + r % 4 of the group.
@@ -207,7 +345,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_few_kernel(const MxLinear a) {
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) c[t][ks] = mx_block(a.w, base + 16 * (col >> 2) + 4 * t + (col & 3), 4 * ks + q, s[t][ks]);
+            for (int ks = 0; ks < KS; ks++) c[t][ks] = mx_operand(a.w, [&](int r) { return base + 16 * (r >> 2) + 4 * t + (r & 3); }, 4 * ks, s[t][ks]);
         float v[16];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
@@ -232,48 +370,83 @@ __global__ __launch_bounds__(MX_T) void mx_linear_few_kernel(const MxLinear a) {
     }
 }
 
+// A block's ROWS x NB tile of results out of LDS (rows of NB + 4 floats), 16 threads and more a row, so that a store instruction writes whole lines: out of the matrix
+// instruction's registers a lane's neighbours belong to other rows, and every 16 bytes were a transaction of their own.
+template <int DT, int ROWS, int NB>
+__device__ __forceinline__ void mx_store_tile(const float* tile, void* y, long long M, long long N, const float* bias, int relu, long long m0, long long m_step, long long n0) {
+    constexpr int TPR = NB / 8, RP = MX_T / TPR;
+    const int c = threadIdx.x % TPR, r0 = threadIdx.x / TPR;
+    const long long n = n0 + c * 8;
+    const int valid = mx_left(n, N);
+    if (valid == 0) return;
+    float b[8];
+    if (bias) vhap_load8(bias, n, VHAP_DTYPE_F32, valid, b);
+#pragma unroll
+    for (int r = r0; r < ROWS; r += RP) {
+        const long long m = m0 + (r & 15) + (r >> 4) * m_step;    // (sixteen consecutive rows at a time)
+        if (m >= M) continue;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + r * (NB + 4) + c * 8), hi = *reinterpret_cast<const f32x4*>(tile + r * (NB + 4) + c * 8 + 4);
+        float o[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (bias) o[e] += b[e];
+            if (relu) o[e] = o[e] < 0.f ? 0.f : o[e];             // (a NaN stays)
+        }
+        vhap_store8(y, m * N + n, DT, valid, o);
+    }
+}
+
 // Any size: a block of four waves owns 64 NT rows of W and 16 CT rows of x; per 128 elements of K the x tile is cut into its pieces once, in LDS, in the
 // order in which the matrix instruction's lanes read it, and every wave multiplies its NT tiles of decoded W with it.
 template <int DT, int NT, int CT>
 __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long long mtiles) {
-    constexpr int P = mx_pieces<DT>();
-    __shared__ bf16x8 xs[CT][4][P][64];
-    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, q = lane >> 4;
+    constexpr int P = mx_pieces<DT>(), NB = 64 * NT;
+    constexpr size_t XS = sizeof(bf16x8) * CT * 4 * P * 64, YS = sizeof(float) * 16 * (NB + 4);
+    __shared__ __attribute__((aligned(16))) unsigned char lds[XS > YS ? XS : YS];
+    auto xs = reinterpret_cast<bf16x8(*)[4][P][64]>(lds);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, q = lane >> 4;
     const long long m0 = (blockIdx.x % mtiles) * 16 * CT;                    // (blocks that share a tile of W run side by side)
-    const long long base = (blockIdx.x / mtiles) * 64 * NT + (tid >> 6) * 16 * NT;
+    const long long n0 = (blockIdx.x / mtiles) * NB, base = n0 + wave * 16 * NT;
     f32x4 acc[NT][CT];
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) acc[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int ks = 0; ks * 128 < a.w.K; ks++) {
-        uint4 c[NT];
-        unsigned s[NT];
+    // the next 128 elements of K are on their way while these are multiplied
+    uint4 c[NT];
+    unsigned s[NT];
+    MxRaw8<DT> xv[CT];
+    const int xr = tid >> 4, xk = (tid & 15) * 8;                            // sixteen threads a row of x, eight elements each
+    auto fetch = [&](int ks) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) c[t] = mx_block(a.w, base + 4 * NT * (col >> 2) + 4 * t + (col & 3), 4 * ks + q, s[t]);
-        if (tid < 64 * CT) {                                                 // four threads a row of x, 32 elements each
-            const int r = tid >> 2, qx = tid & 3;
+        for (int t = 0; t < NT; t++) c[t] = mx_block(a.w, base + 16 * t + (lane >> 2), 4 * ks + (lane & 3), s[t]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int k0 = 128 * ks + 32 * qx + 8 * j;
-                float v[8];
-                bf16x8 f[P];
-                vhap_load8(a.x, (m0 + r) * a.ldx + k0, DT, m0 + r < a.M ? mx_left(k0, a.w.K) : 0, v);
-                mx_split8<P>(v, f);
-#pragma unroll
-                for (int p = 0; p < P; p++) xs[r >> 4][j][p][qx * 16 + (r & 15)] = f[p];
-            }
+        for (int ct = 0; ct < CT; ct++) {
+            const long long m = m0 + 16 * ct + xr;
+            mx_load_raw8<DT>(a.x, m * a.ldx + 128 * ks + xk, m < a.M ? mx_left(128 * ks + xk, a.w.K) : 0, xv[ct]);
         }
-        __syncthreads();
+    };
+    const int from = 4 * (4 * col + q);                                      // (mx_operand, with the loads ahead of their use)
+    fetch(0);
+    for (int ks = 0; ks * 128 < a.w.K; ks++) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            bf16x8 f[P];
+            mx_fragments<DT>(xv[ct], f);
+#pragma unroll
+            for (int p = 0; p < P; p++) xs[ct][(tid & 15) & 3][p][((tid & 15) >> 2) * 16 + xr] = f[p];
+        }
         bf16x8 w[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const float sc = mx_scale(s[t]);
-            w[t][0] = mx_decode8(c[t].x, sc);
-            w[t][1] = mx_decode8(c[t].y, sc);
-            w[t][2] = mx_decode8(c[t].z, sc);
-            w[t][3] = mx_decode8(c[t].w, sc);
+            const float sc = mx_scale((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)s[t]));
+            w[t][0] = mx_decode8((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c[t].x), sc);
+            w[t][1] = mx_decode8((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c[t].y), sc);
+            w[t][2] = mx_decode8((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c[t].z), sc);
+            w[t][3] = mx_decode8((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c[t].w), sc);
         }
+        __syncthreads();
+        if ((ks + 1) * 128 < a.w.K) fetch(ks + 1);
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -286,15 +459,14 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
                 }
         __syncthreads();
     }
+    float* tile = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        const long long m = m0 + 16 * ct + col;
-        float v[NT * 4];
+        if (ct) __syncthreads();
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[4 * t + i] = acc[t][ct][i];
-        if (m < a.M) mx_store_row<DT, NT>(a, m, base + 4 * NT * q, v);
+        for (int t = 0; t < NT; t++) *reinterpret_cast<f32x4*>(tile + col * (NB + 4) + wave * 16 * NT + 16 * t + 4 * q) = acc[t][ct];
+        __syncthreads();
+        mx_store_tile<DT, 16, NB>(tile, a.y, a.M, a.w.rows, a.bias, 0, m0 + 16 * ct, 0, n0);
     }
 }
 
@@ -335,26 +507,18 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_few_kernel(const MxInputGr
                 g[u][m] = 0.f;
                 if (row < a.w.rows && m < a.M) {
                     const long long at = m * a.ldg + row;
-                    if constexpr (DT == VHAP_DTYPE_F32) g[u][m] = static_cast<const float*>(a.g)[at];
-                    if constexpr (DT == VHAP_DTYPE_BF16) g[u][m] = __uint_as_float((unsigned)static_cast<const unsigned short*>(a.g)[at] << 16);
-                    if constexpr (DT == VHAP_DTYPE_F16) g[u][m] = __half2float(static_cast<const __half*>(a.g)[at]);
+                    g[u][m] = mx_one<DT>(a.g, at);
                 }
             }
         }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const float sc = mx_scale(s[u]);
-            const unsigned w4[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+            float w[32];
+            mx_decode32(c[u], mx_scale(s[u]), w);
 #pragma unroll
-            for (int d = 0; d < 4; d++) {
-                const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w4[d], sc, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w4[d], sc, 1);
-                const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w4[d], sc, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w4[d], sc, 3);
-                const float wv[8] = {p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+            for (int m = 0; m < MM; m++)
 #pragma unroll
-                for (int m = 0; m < MM; m++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) acc[m][8 * d + e] = fmaf(wv[e], g[u][m], acc[m][8 * d + e]);
-            }
+                for (int e = 0; e < 32; e++) acc[m][e] = fmaf(w[e], g[u][m], acc[m][e]);
         }
     }
     // the 16 lanes that share a block, then the four waves
@@ -394,25 +558,30 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
         for (int ct = 0; ct < CT; ct++) acc[k][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     const long long n0 = ((long long)blockIdx.x * (MX_T / 64) + wave) * a.steps_per_wave * 32;
     const long long n1 = min(n0 + a.steps_per_wave * 32, a.w.rows);
-    for (long long n = n0; n < n1; n += 32) {
-        unsigned c[8], s[8];
+    unsigned nc[8], ns[8];                                        // the next 32 rows, on their way while these are multiplied
+    MxRaw8<DT> ng[CT];
+    auto fetch = [&](long long n) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const long long row = n + 8 * q + i;
-            const bool ok = row < a.w.rows && blk < a.w.Kb;
-            const size_t at = ok ? (size_t)row * a.w.Kb + blk : 0;
-            c[i] = reinterpret_cast<const unsigned*>(a.w.codes)[at * 4 + (col & 3)];
-            s[i] = a.w.scales[at];
-            if (!ok) { c[i] = 0u; s[i] = 127u; }
+            const size_t at = (size_t)min(n + 8 * q + i, a.w.rows - 1) * a.w.Kb + min(blk, a.w.Kb - 1);
+            nc[i] = reinterpret_cast<const unsigned*>(a.w.codes)[at * 4 + (col & 3)];
+            ns[i] = a.w.scales[at];
         }
-        bf16x8 gb[CT][P];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const long long m = m0 + 16 * ct + col;
-            float v[8];
-            vhap_load8(a.g, m * a.ldg + n + 8 * q, DT, m < a.M ? mx_left(n + 8 * q, a.w.rows) : 0, v);
-            mx_split8<P>(v, gb[ct]);
+            mx_load_raw8<DT>(a.g, m * a.ldg + n + 8 * q, m < a.M ? mx_left(n + 8 * q, a.w.rows) : 0, ng[ct]);
         }
+    };
+    if (n0 < n1) fetch(n0);
+    for (long long n = n0; n < n1; n += 32) {
+        unsigned c[8], s[8];
+        bf16x8 gb[CT][P];
+#pragma unroll
+        for (int i = 0; i < 8; i++) { c[i] = nc[i]; s[i] = ns[i]; }
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) mx_fragments<DT>(ng[ct], gb[ct]);
+        if (n + 32 < n1) fetch(n + 32);
 #pragma unroll
         for (int h = 0; h < 4; h++) {                             // elements 2 h and 2 h + 1
             unsigned pk[8];
@@ -454,51 +623,57 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
     }
 }
 
-// dx[m, k] (+)= sum over the splits, in order: SG threads an element, each a run of splits
-template <int DT, int SG>
-__global__ __launch_bounds__(MX_T) void mx_join_kernel(const float* __restrict__ part, int splits, long long M, int K, int Kp, void* __restrict__ dx, int accumulate) {
-    constexpr int EL = MX_T / SG;
+// dx[m, k] (+)= sum over the splits: SG threads an element, each every SG-th split, joined in order
+template <int DT, int EL, int SG>
+__global__ __launch_bounds__(EL * SG) void mx_join_kernel(const float* __restrict__ part, int splits, long long M, int K, int Kp, void* __restrict__ dx, int accumulate) {
     __shared__ float red[SG][EL];
     const int e = threadIdx.x % EL, sg = threadIdx.x / EL;
     const long long i = (long long)blockIdx.x * EL + e;
     const long long m = i / K;
     const int k = (int)(i - m * K);
     float v = 0.f;
-    if (m < M)
-        for (int s = sg; s < splits; s += SG) v += part[((size_t)s * M + m) * Kp + k];
+    if (m < M) {
+        const float* p = part + m * Kp + k;
+#pragma unroll 8
+        for (int s = sg; s < splits; s += SG) v += p[(size_t)s * M * Kp];
+    }
     red[sg][e] = v;
     __syncthreads();
     if (sg == 0 && m < M) {
+#pragma unroll 8
         for (int j = 1; j < SG; j++) v += red[j][e];
-        if constexpr (DT == VHAP_DTYPE_F32) {
-            float* o = static_cast<float*>(dx) + i;
-            *o = accumulate ? *o + v : v;
-        }
-        if constexpr (DT == VHAP_DTYPE_BF16) static_cast<unsigned short*>(dx)[i] = (unsigned short)vhap_bf16_bits(v);
-        if constexpr (DT == VHAP_DTYPE_F16) static_cast<__half*>(dx)[i] = __float2half_rn(v);
+        if (DT == VHAP_DTYPE_F32 && accumulate) v = static_cast<float*>(dx)[i] + v;
+        mx_put<DT>(dx, i, v);
     }
 }
 
-// db[n] = sum_m g[m, n]: 64 columns x 16 runs of rows a block
-template <int DT>
-__global__ __launch_bounds__(1024) void mx_colsum_kernel(const void* __restrict__ g, long long ldg, long long M, long long N, float* __restrict__ out) {
-    __shared__ float red[16][64];
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-    const long long n = (long long)blockIdx.x * 64 + c;
-    float v = 0.f;
-    if (n < N)
-        for (long long m = r; m < M; m += 16) {
-            const long long at = m * ldg + n;
-            if constexpr (DT == VHAP_DTYPE_F32) v += static_cast<const float*>(g)[at];
-            if constexpr (DT == VHAP_DTYPE_BF16) v += __uint_as_float((unsigned)static_cast<const unsigned short*>(g)[at] << 16);
-            if constexpr (DT == VHAP_DTYPE_F16) v += __half2float(static_cast<const __half*>(g)[at]);
+// db[n] = sum_m g[m, n]: RG runs of rows x 256 / RG threads of eight columns a block, the runs joined in order
+template <int DT, int RG>
+__global__ __launch_bounds__(MX_T) void mx_colsum_kernel(const void* __restrict__ g, long long ldg, long long M, long long N, float* __restrict__ out) {
+    constexpr int CG = MX_T / RG;
+    __shared__ float red[RG > 1 ? RG : 1][RG > 1 ? CG : 1][8 + 1];
+    const int c = threadIdx.x % CG, r = threadIdx.x / CG;
+    const long long n = ((long long)blockIdx.x * CG + c) * 8;
+    const int valid = mx_left(n, N);
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (valid)
+#pragma unroll 4
+        for (long long m = r; m < M; m += RG) {
+            float x[8];
+            vhap_load8(g, m * ldg + n, DT, valid, x);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] += x[e];
         }
-    red[r][c] = v;
-    __syncthreads();
-    if (r == 0 && n < N) {
-        for (int j = 1; j < 16; j++) v += red[j][c];
-        out[n] = v;
+    if constexpr (RG > 1) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) red[r][c][e] = v[e];
+        __syncthreads();
+        if (r > 0) return;
+        for (int j = 1; j < RG; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] += red[j][c][e];
     }
+    if (valid) vhap_store8(out, n, VHAP_DTYPE_F32, valid, v);
 }
 
 // ---- matmul: both operands in 4 bits ----
@@ -509,33 +684,88 @@ struct MxMatmul {
     void* y;                  // [M, N]
 };
 
-// A wave owns 64 rows of B x 64 rows of A (4 x 4 tiles of the scaled 16 x 16 x 128 instruction), a block of four waves 128 x 128; B's rows are dealt out as in
-// mx_linear_few_kernel, so that a lane writes 16 consecutive columns of a row of y.
+// A block of four waves owns 128 rows of B x 128 rows of A, a wave 64 x 64 of them (4 x 4 tiles of the scaled 16 x 16 x 128 instruction).  128 elements of K -- 64
+// bytes and four scale bytes a row -- go through LDS at a time, double-buffered, the next ones on their way in registers while these are multiplied: every
+// row is read once a block instead of twice.
+struct MxTile {
+    uint4 codes[128][4];      // block q of row r at place mx_place(r, q): eight neighbouring lanes, which read eight rows' block q, meet eight different places modulo 128 bytes
+    unsigned scales[128];     // four blocks' bytes
+};
+__device__ __forceinline__ int mx_place(int row, int q) { return q ^ ((row >> 1) & 3); }
+
+// a row's four scale bytes of blocks k .. k + 3 (behind the last block: scale 1)
+__device__ __forceinline__ unsigned mx_scales4(const uint8_t* row, int k, int Kb) {
+    if (k + 4 <= Kb) {                                            // (the same for the whole block of threads)
+        struct __attribute__((packed)) Bytes4 { unsigned v; };
+        return reinterpret_cast<const Bytes4*>(row + k)->v;
+    }
+    unsigned s = 0x7f7f7f7fu;
+    for (int b = 0; k + b < Kb; b++) s = (s & ~(0xffu << 8 * b)) | (unsigned)row[k + b] << 8 * b;
+    return s;
+}
+
 template <int DT>
 __global__ __launch_bounds__(MX_T) void mx_matmul_kernel(const MxMatmul a, long long mtiles) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q = lane >> 4;
-    const long long m0 = (blockIdx.x % mtiles) * 128 + (wave & 1) * 64;
-    const long long n0 = (blockIdx.x / mtiles) * 128 + (wave >> 1) * 64;
+    __shared__ MxTile ta[2], tb[2];
+    const unsigned tid = threadIdx.x;
+    const int lane = tid & 63, wave = tid >> 6, col = lane & 15, q = lane >> 4;
+    const long long m0 = (blockIdx.x % mtiles) * 128, n0 = (blockIdx.x / mtiles) * 128;
+    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
     f32x4 acc[4][4];
 #pragma unroll
     for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int u = 0; u < 4; u++) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int last = a.b.K & 31;                                  // elements of the last block, 0: all
-    for (int k = 0; k < a.b.Kb; k += 4) {
-        uint4 bc[4], ac[4];
-        unsigned bs[4], as[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            bc[t] = mx_block(a.b, n0 + 16 * (col >> 2) + 4 * t + (col & 3), k + q, bs[t]);
-            ac[t] = mx_block(a.a, m0 + 16 * t + col, k + q, as[t]);
-        }
-        if (last && k + q == a.b.Kb - 1) {                        // codes behind K count as zero, whatever they hold
+    // this thread's pieces of the tiles: block `blk` of rows tid / 4 and 64 further of A and of B, and the four scale bytes of a row of A (threads 0 .. 127) or of B.
+    // Rows behind the last are the last one's (their results are not stored).
+    const int Kb = a.b.Kb, last = a.b.K & 31, r0 = tid >> 2, blk = tid & 3;
+    auto row_at = [](const MxMatrix& w, long long row) { return (size_t)min(row, w.rows - 1) * w.Kb; };
+    const uint4* const a0 = reinterpret_cast<const uint4*>(a.a.codes) + row_at(a.a, m0 + r0);
+    const uint4* const a1 = reinterpret_cast<const uint4*>(a.a.codes) + row_at(a.a, m0 + 64 + r0);
+    const uint4* const b0 = reinterpret_cast<const uint4*>(a.b.codes) + row_at(a.b, n0 + r0);
+    const uint4* const b1 = reinterpret_cast<const uint4*>(a.b.codes) + row_at(a.b, n0 + 64 + r0);
+    const uint8_t* const sr = tid < 128 ? a.a.scales + row_at(a.a, m0 + tid) : a.b.scales + row_at(a.b, n0 + tid - 128);
+    const int p0 = mx_place(r0, blk);                             // (the same place in row r0 + 64)
+    uint4 ca0, ca1, cb0, cb1;
+    unsigned sc;
+    auto fetch = [&](int k) {
+        const int at = min(k + blk, Kb - 1);
+        ca0 = a0[at];
+        ca1 = a1[at];
+        cb0 = b0[at];
+        cb1 = b1[at];
+        sc = mx_scales4(sr, k, Kb);
+    };
+    auto put = [&](int buf, int k) {
+        if (k + 4 >= Kb) {                                        // the last round: codes behind K are zero in one operand, whatever the matrix holds there
+            const int left = k + blk < Kb - 1 ? 32 : k + blk == Kb - 1 ? (last ? last : 32) : 0;
             unsigned mask[4];
 #pragma unroll
-            for (int d = 0; d < 4; d++) mask[d] = last >= 8 * d + 8 ? ~0u : last <= 8 * d ? 0u : (1u << 4 * (last - 8 * d)) - 1u;
+            for (int d = 0; d < 4; d++) mask[d] = left >= 8 * d + 8 ? ~0u : left <= 8 * d ? 0u : (1u << 4 * (left - 8 * d)) - 1u;
+            cb0.x &= mask[0]; cb0.y &= mask[1]; cb0.z &= mask[2]; cb0.w &= mask[3];
+            cb1.x &= mask[0]; cb1.y &= mask[1]; cb1.z &= mask[2]; cb1.w &= mask[3];
+        }
+        ta[buf].codes[r0][p0] = ca0;
+        ta[buf].codes[r0 + 64][p0] = ca1;
+        tb[buf].codes[r0][p0] = cb0;
+        tb[buf].codes[r0 + 64][p0] = cb1;
+        (tid < 128 ? ta : tb)[buf].scales[tid & 127] = sc;
+    };
+    fetch(0);
+    put(0, 0);
+    __syncthreads();
+    for (int k = 0, buf = 0; k < Kb; k += 4, buf ^= 1) {
+        const bool more = k + 4 < Kb;
+        if (more) fetch(k + 4);
+        uint4 bc[4], ac[4];
+        int bs[4], as[4];
 #pragma unroll
-            for (int t = 0; t < 4; t++) { bc[t].x &= mask[0]; bc[t].y &= mask[1]; bc[t].z &= mask[2]; bc[t].w &= mask[3]; }
+        for (int t = 0; t < 4; t++) {
+            const int rb = wn + 16 * t + col, ra = wm + 16 * t + col;
+            bc[t] = tb[buf].codes[rb][mx_place(rb, q)];
+            bs[t] = (int)(tb[buf].scales[rb] >> 8 * q);
+            ac[t] = ta[buf].codes[ra][mx_place(ra, q)];
+            as[t] = (int)(ta[buf].scales[ra] >> 8 * q);
         }
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -543,28 +773,21 @@ __global__ __launch_bounds__(MX_T) void mx_matmul_kernel(const MxMatmul a, long 
             for (int u = 0; u < 4; u++) {
                 const i32x8 x = {(int)bc[t].x, (int)bc[t].y, (int)bc[t].z, (int)bc[t].w, 0, 0, 0, 0};
                 const i32x8 y = {(int)ac[u].x, (int)ac[u].y, (int)ac[u].z, (int)ac[u].w, 0, 0, 0, 0};
-                acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, acc[t][u], 4, 4, 0, (int)bs[t], 0, (int)as[u]);
+                acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, acc[t][u], 4, 4, 0, bs[t], 0, as[u]);     // (the low byte of the scale operands)
             }
+        __builtin_amdgcn_sched_barrier(0);     // (the loads are waited for here, behind the products, not in front of them)
+        if (more) put(buf ^ 1, k + 4);         // (the other buffer: its readers passed the barrier of the round before)
+        __syncthreads();
     }
+    float* tile = reinterpret_cast<float*>(ta);                   // 32 rows of 128 + 4 floats: half of the two buffers
+    static_assert(sizeof(float) * 32 * 132 <= sizeof(MxTile) * 2, "the results' tile fits the operands' buffers");
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-        const long long m = m0 + 16 * u + col;
-        if (m >= a.a.rows) continue;
+        if (u) __syncthreads();
 #pragma unroll
-        for (int h = 0; h < 16; h += 8) {
-            const long long n = n0 + 16 * q + h;
-            const int valid = mx_left(n, a.b.rows);
-            if (valid == 0) continue;
-            float o[8], b[8];
-            if (a.bias) vhap_load8(a.bias, n, VHAP_DTYPE_F32, valid, b);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                o[e] = acc[(h + e) >> 2][u][e & 3];
-                if (a.bias) o[e] += b[e];
-                if (a.relu) o[e] = o[e] < 0.f ? 0.f : o[e];       // (a NaN stays)
-            }
-            vhap_store8(a.y, m * a.b.rows + n, DT, valid, o);
-        }
+        for (int t = 0; t < 4; t++) *reinterpret_cast<f32x4*>(tile + ((wave & 1) * 16 + col) * 132 + wn + 16 * t + 4 * q) = acc[t][u];
+        __syncthreads();
+        mx_store_tile<DT, 32, 128>(tile, a.y, a.a.rows, a.b.rows, a.bias, a.relu, m0 + 16 * u, 64, n0);
     }
 }
 
@@ -605,6 +828,17 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
     constexpr int P = mx_pieces<DT>();
     const long long N = a.w.rows;
     const int ks = (a.w.K + 127) / 128;
+    if (a.M <= 2 && ks <= (a.M == 1 ? 4 : 2)) {
+        const int grid = mx_grid((N + 63) / 64 * 64, 2048);
+        if (a.M == 2) {
+            if (ks == 1) mx_linear_row_kernel<DT, 2, 1><<<grid, MX_T, 0, st>>>(a);
+            else mx_linear_row_kernel<DT, 2, 2><<<grid, MX_T, 0, st>>>(a);
+        } else if (ks == 1) mx_linear_row_kernel<DT, 1, 1><<<grid, MX_T, 0, st>>>(a);
+        else if (ks == 2) mx_linear_row_kernel<DT, 1, 2><<<grid, MX_T, 0, st>>>(a);
+        else mx_linear_row_kernel<DT, 1, 4><<<grid, MX_T, 0, st>>>(a);
+        VHAP_LAUNCH_CHECK();
+        return VHAP_OK;
+    }
     if (a.M * P <= 16 && ks <= 4) {
         const int grid = mx_grid((N + 63) / 64 * 64, 2048);
         if (ks == 1) mx_linear_few_kernel<DT, 1><<<grid, MX_T, 0, st>>>(a);
@@ -641,8 +875,9 @@ int mx_input_grad_launch(const MxInputGrad& a, const GradPlan& p, void* dx, int 
     else mx_input_grad_kernel<DT, 4><<<grid, MX_T, 0, st>>>(a);
     VHAP_LAUNCH_CHECK();
     const long long n = a.M * a.w.K;
-    if (p.splits > 64) mx_join_kernel<DT, 32><<<vhap_cdiv(n, MX_T / 32), MX_T, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
-    else mx_join_kernel<DT, 4><<<vhap_cdiv(n, MX_T / 4), MX_T, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
+    // many splits of few elements: 64 threads an element; else four
+    if (p.splits > 64) mx_join_kernel<DT, 16, 64><<<vhap_cdiv(n, 16), 1024, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
+    else mx_join_kernel<DT, 64, 4><<<vhap_cdiv(n, 64), 256, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
 }
@@ -698,7 +933,7 @@ extern "C" int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ld
     if (M == 0) return VHAP_OK;
     if (!g || !codes || !scales || !dx || !workspace) return VHAP_E_NULLPTR;
     const GradPlan p = mx_grad_plan(M, N, K);
-    if (p.ktiles > 65535 || p.mtiles > 65535 || M * K / (MX_T / 32) >= (1ll << 31)) return VHAP_E_BADDIM;
+    if (p.ktiles > 65535 || p.mtiles > 65535 || M * K / 16 >= (1ll << 31) - 1) return VHAP_E_BADDIM;
     if (workspace_bytes < vhap_mx4_linear_input_grad_workspace_bytes(M, N, K)) return VHAP_E_WORKSPACE;
     const MxInputGrad a{g, ldg, M, {codes, scales, N, K, mx_kb(K)}, static_cast<float*>(workspace), p.ktiles, p.steps_per_wave};
     int rc = VHAP_OK;
@@ -708,10 +943,12 @@ extern "C" int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ld
 
 extern "C" int vhap_mx4_column_sums(const void* g, int dtype, long long ldg, long long M, long long N, float* out, vhap_stream_t stream) {
     VHAP_ENTER();
-    if (!mx_dims(M, 1) || !mx_dims(N, 1) || !mx_dt(dtype) || ldg < 0 || (N + 63) / 64 >= (1ll << 31)) return VHAP_E_BADDIM;
+    if (!mx_dims(M, 1) || !mx_dims(N, 1) || !mx_dt(dtype) || ldg < 0 || N / 64 >= (1ll << 31) - 1) return VHAP_E_BADDIM;
     if (N == 0) return VHAP_OK;
     if (!out || (M > 0 && !g)) return VHAP_E_NULLPTR;
-    MX_BY_TYPE(dtype, (mx_colsum_kernel<DT><<<(int)((N + 63) / 64), 1024, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)));
+    // few rows: every thread sums its own columns; from eight rows on 32 threads share them (64 columns a block)
+    if (M < 8) MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 1><<<vhap_cdiv(N, 8 * MX_T), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)))
+    else MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 32><<<vhap_cdiv(N, 8 * MX_T / 32), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)));
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
 }
