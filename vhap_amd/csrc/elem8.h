@@ -44,10 +44,13 @@ __device__ __forceinline__ void vhap_load8(const void* p, long long i, int dt, i
     }
 }
 
-__device__ __forceinline__ unsigned vhap_bf16_bits(float f) {           // to nearest even; a NaN keeps its sign and stays one
-    const unsigned u = __float_as_uint(f);
-    return (u & 0x7fffffffu) > 0x7f800000u ? (u >> 16 | 0x40u) : (u + 0x7fffu + (u >> 16 & 1)) >> 16;
+// to nearest, halves to even; a NaN stays one (the target's own conversion, two numbers an instruction)
+typedef __bf16 vhap_bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned vhap_bf16_pair(float lo, float hi) {
+    const vhap_bf16x2 v = {(__bf16)lo, (__bf16)hi};
+    return __builtin_bit_cast(unsigned, v);
 }
+__device__ __forceinline__ unsigned vhap_bf16_bits(float f) { return vhap_bf16_pair(f, f) & 0xffffu; }
 
 __device__ __forceinline__ void vhap_store8(void* p, long long i, int dt, int valid, const float (&v)[8]) {
     if (dt == VHAP_DTYPE_F32) {
@@ -65,18 +68,20 @@ __device__ __forceinline__ void vhap_store8(void* p, long long i, int dt, int va
         }
         return;
     }
-    unsigned h[8];
+    unsigned h[4];
 #pragma unroll
-    for (int k = 0; k < 8; k++) h[k] = dt == VHAP_DTYPE_BF16 ? vhap_bf16_bits(v[k]) : (unsigned)__half_as_ushort(__float2half_rn(v[k]));
+    for (int k = 0; k < 4; k++)
+        h[k] = dt == VHAP_DTYPE_BF16 ? vhap_bf16_pair(v[2 * k], v[2 * k + 1])
+                                     : (unsigned)__half_as_ushort(__float2half_rn(v[2 * k])) | (unsigned)__half_as_ushort(__float2half_rn(v[2 * k + 1])) << 16;
     unsigned short* q = static_cast<unsigned short*>(p) + i;
     if (valid >= 8) {
         VhapVec16a2 a;
 #pragma unroll
-        for (int k = 0; k < 4; k++) a.w[k] = h[2 * k] | h[2 * k + 1] << 16;
+        for (int k = 0; k < 4; k++) a.w[k] = h[k];
         *reinterpret_cast<VhapVec16a2*>(q) = a;
     } else {
 #pragma unroll
         for (int k = 0; k < 8; k++)
-            if (k < valid) q[k] = (unsigned short)h[k];
+            if (k < valid) q[k] = (unsigned short)(h[k >> 1] >> 16 * (k & 1));
     }
 }

@@ -25,6 +25,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));      // (HIP's uint4 holds a union: arrays of it end up in scratch memory)
 
 constexpr int MX_T = 256;
 
@@ -40,20 +41,20 @@ __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_floa
 // the 16 bytes of codes and the scale byte of block `blk` of `row`; behind the last row or block: the last one's, without a branch around the load.  Nothing is wrong with that
 // where the other operand is zero behind the last block (or row, in the input's gradient) and results behind the last row are not stored: a product with zero is
 // zero, or NaN where that last block is NaN and the sum is NaN already.
-__device__ __forceinline__ uint4 mx_block(const MxMatrix& w, long long row, int blk, unsigned& scale) {
+__device__ __forceinline__ u32x4 mx_block(const MxMatrix& w, long long row, int blk, unsigned& scale) {
     const size_t at = (size_t)min(row, w.rows - 1) * w.Kb + min(blk, w.Kb - 1);
     scale = w.scales[at];
-    return reinterpret_cast<const uint4*>(w.codes)[at];
+    return reinterpret_cast<const u32x4*>(w.codes)[at];
 }
 
 // The same for a matrix instruction's operand: lane (r, q) = (lane % 16, lane / 16) gets block k + q of row row_of(r).  Read in that order, sixteen neighbouring lanes would
 // touch sixteen rows, four times over; read four lanes a row and passed on across the wave, neighbours read 64 consecutive bytes.
 template <typename F>
-__device__ __forceinline__ uint4 mx_operand(const MxMatrix& w, F row_of, int k, unsigned& scale) {
+__device__ __forceinline__ u32x4 mx_operand(const MxMatrix& w, F row_of, int k, unsigned& scale) {
     const int lane = threadIdx.x & 63, from = 4 * (4 * (lane & 15) + (lane >> 4));
-    const uint4 c = mx_block(w, row_of(lane >> 2), k + (lane & 3), scale);
+    const u32x4 c = mx_block(w, row_of(lane >> 2), k + (lane & 3), scale);
     scale = (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)scale);
-    return uint4{(unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.x), (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.y),
+    return u32x4{(unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.x), (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.y),
                  (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.z), (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.w)};
 }
 
@@ -61,7 +62,7 @@ __device__ __forceinline__ unsigned mx_pair_bits(bf16x2 v) { return __builtin_bi
 
 // eight codes (one dword) -> eight bf16 numbers
 __device__ __forceinline__ bf16x8 mx_decode8(unsigned codes, float scale) {
-    uint4 r;
+    u32x4 r;
     r.x = mx_pair_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
     r.y = mx_pair_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
     r.z = mx_pair_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
@@ -96,7 +97,7 @@ __device__ __forceinline__ void mx_split8(const float (&v)[8], bf16x8 (&out)[P])
     for (int e = 0; e < 8; e++) mx_split<P>(v[e], t[e]);
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        uint4 r;
+        u32x4 r;
         r.x = t[0][p] >> 16 | t[1][p];
         r.y = t[2][p] >> 16 | t[3][p];
         r.z = t[4][p] >> 16 | t[5][p];
@@ -108,29 +109,29 @@ __device__ __forceinline__ void mx_split8(const float (&v)[8], bf16x8 (&out)[P])
 // eight elements as they lie in memory: a load that is to be in flight under other work must not be converted where it is issued
 template <int DT>
 struct MxRaw8 {
-    unsigned w[DT == VHAP_DTYPE_F32 ? 8 : 4];
+    u32x4 lo, hi;             // (hi: float32 only)
 };
 template <int DT>
 __device__ __forceinline__ void mx_load_raw8(const void* p, long long i, int valid, MxRaw8<DT>& r) {
     if constexpr (DT == VHAP_DTYPE_F32) {
         const float* q = static_cast<const float*>(p) + i;
         if (valid >= 8) {
-            const VhapVec16a4 a = *reinterpret_cast<const VhapVec16a4*>(q), b = *reinterpret_cast<const VhapVec16a4*>(q + 4);
-#pragma unroll
-            for (int k = 0; k < 4; k++) { r.w[k] = a.w[k]; r.w[4 + k] = b.w[k]; }
+            typedef u32x4 __attribute__((aligned(4))) at4;
+            r.lo = *reinterpret_cast<const at4*>(q);
+            r.hi = *reinterpret_cast<const at4*>(q + 4);
         } else {
-#pragma unroll
-            for (int k = 0; k < 8; k++) r.w[k] = k < valid ? __float_as_uint(q[k]) : 0u;
+            const unsigned* u = reinterpret_cast<const unsigned*>(q);
+            r.lo = u32x4{valid > 0 ? u[0] : 0u, valid > 1 ? u[1] : 0u, valid > 2 ? u[2] : 0u, valid > 3 ? u[3] : 0u};
+            r.hi = u32x4{valid > 4 ? u[4] : 0u, valid > 5 ? u[5] : 0u, valid > 6 ? u[6] : 0u, 0u};
         }
     } else {
         const unsigned short* q = static_cast<const unsigned short*>(p) + i;
         if (valid >= 8) {
-            const VhapVec16a2 a = *reinterpret_cast<const VhapVec16a2*>(q);
-#pragma unroll
-            for (int k = 0; k < 4; k++) r.w[k] = a.w[k];
+            typedef u32x4 __attribute__((aligned(2))) at2;
+            r.lo = *reinterpret_cast<const at2*>(q);
         } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++) r.w[k] = (2 * k < valid ? (unsigned)q[2 * k] : 0u) | (2 * k + 1 < valid ? (unsigned)q[2 * k + 1] << 16 : 0u);
+            auto two = [&](int k) { return (k < valid ? (unsigned)q[k] : 0u) | (k + 1 < valid ? (unsigned)q[k + 1] << 16 : 0u); };
+            r.lo = u32x4{two(0), two(2), two(4), two(6)};
         }
     }
 }
@@ -138,13 +139,18 @@ __device__ __forceinline__ void mx_load_raw8(const void* p, long long i, int val
 template <int DT>
 __device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[mx_pieces<DT>()]) {
     if constexpr (DT == VHAP_DTYPE_BF16) {
-        out[0] = __builtin_bit_cast(bf16x8, r);
+        out[0] = __builtin_bit_cast(bf16x8, r.lo);
     } else {
         float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            if constexpr (DT == VHAP_DTYPE_F32) v[k] = __uint_as_float(r.w[k]);
-            else v[k] = __half2float(__ushort_as_half((unsigned short)(r.w[k >> 1] >> 16 * (k & 1))));
+        for (int k = 0; k < 4; k++) {
+            if constexpr (DT == VHAP_DTYPE_F32) {
+                v[k] = __uint_as_float(r.lo[k]);
+                v[4 + k] = __uint_as_float(r.hi[k]);
+            } else {
+                v[2 * k] = __half2float(__ushort_as_half((unsigned short)(r.lo[k] & 0xffffu)));
+                v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(r.lo[k] >> 16)));
+            }
         }
         mx_split8<mx_pieces<DT>()>(v, out);
     }
@@ -242,7 +248,7 @@ __device__ __forceinline__ void mx_put(void* p, long long i, float v) {
     if constexpr (DT == VHAP_DTYPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 // the 32 numbers of a block, scaled
-__device__ __forceinline__ void mx_decode32(const uint4& c, float scale, float (&v)[32]) {
+__device__ __forceinline__ void mx_decode32(const u32x4& c, float scale, float (&v)[32]) {
     const unsigned w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int d = 0; d < 4; d++) {
@@ -273,7 +279,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_row_kernel(const MxLinear a) {
             }
     const long long groups = (a.w.rows + 63) / 64;
     for (long long g = (long long)blockIdx.x * (MX_T / 64) + (threadIdx.x >> 6); g < groups; g += (long long)gridDim.x * (MX_T / 64)) {
-        uint4 c[4][KS];
+        u32x4 c[4][KS];
         unsigned s[4][KS];
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -340,7 +346,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_few_kernel(const MxLinear a) {
     const long long groups = (a.w.rows + 63) / 64;
     for (long long g = (long long)blockIdx.x * (MX_T / 64) + (threadIdx.x >> 6); g < groups; g += (long long)gridDim.x * (MX_T / 64)) {
         const long long base = g * 64;
-        uint4 c[4][KS];
+        u32x4 c[4][KS];
         unsigned s[4][KS];
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -372,9 +378,9 @@ __global__ __launch_bounds__(MX_T) void mx_linear_few_kernel(const MxLinear a) {
 
 // A block's ROWS x NB tile of results out of LDS (rows of NB + 4 floats), 16 threads and more a row, so that a store instruction writes whole lines: out of the matrix
 // instruction's registers a lane's neighbours belong to other rows, and every 16 bytes were a transaction of their own.
-template <int DT, int ROWS, int NB>
+template <int DT, int T, int ROWS, int NB>
 __device__ __forceinline__ void mx_store_tile(const float* tile, void* y, long long M, long long N, const float* bias, int relu, long long m0, long long m_step, long long n0) {
-    constexpr int TPR = NB / 8, RP = MX_T / TPR;
+    constexpr int TPR = NB / 8, RP = T / TPR;
     const int c = threadIdx.x % TPR, r0 = threadIdx.x / TPR;
     const long long n = n0 + c * 8;
     const int valid = mx_left(n, N);
@@ -413,7 +419,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) acc[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     // the next 128 elements of K are on their way while these are multiplied
-    uint4 c[NT];
+    u32x4 c[NT];
     unsigned s[NT];
     MxRaw8<DT> xv[CT];
     const int xr = tid >> 4, xk = (tid & 15) * 8;                            // sixteen threads a row of x, eight elements each
@@ -466,7 +472,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
 #pragma unroll
         for (int t = 0; t < NT; t++) *reinterpret_cast<f32x4*>(tile + col * (NB + 4) + wave * 16 * NT + 16 * t + 4 * q) = acc[t][ct];
         __syncthreads();
-        mx_store_tile<DT, 16, NB>(tile, a.y, a.M, a.w.rows, a.bias, 0, m0 + 16 * ct, 0, n0);
+        mx_store_tile<DT, MX_T, 16, NB>(tile, a.y, a.M, a.w.rows, a.bias, 0, m0 + 16 * ct, 0, n0);
     }
 }
 
@@ -495,7 +501,7 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_few_kernel(const MxInputGr
     const long long n0 = ((long long)blockIdx.x * (MX_T / 64) + wave) * a.steps_per_wave * 32;
     const long long n1 = min(n0 + a.steps_per_wave * 32, a.w.rows);
     for (long long n = n0; n < n1; n += 32) {
-        uint4 c[2];
+        u32x4 c[2];
         unsigned s[2];
         float g[2][MM];
 #pragma unroll
@@ -593,9 +599,9 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
                         : h == 2 ? mx_pair_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[i], sc, 2))
                                  : mx_pair_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[i], sc, 3));
             }
-            const uint4 even = {__builtin_amdgcn_perm(pk[1], pk[0], 0x05040100), __builtin_amdgcn_perm(pk[3], pk[2], 0x05040100),
+            const u32x4 even = {__builtin_amdgcn_perm(pk[1], pk[0], 0x05040100), __builtin_amdgcn_perm(pk[3], pk[2], 0x05040100),
                                 __builtin_amdgcn_perm(pk[5], pk[4], 0x05040100), __builtin_amdgcn_perm(pk[7], pk[6], 0x05040100)};
-            const uint4 odd = {__builtin_amdgcn_perm(pk[1], pk[0], 0x07060302), __builtin_amdgcn_perm(pk[3], pk[2], 0x07060302),
+            const u32x4 odd = {__builtin_amdgcn_perm(pk[1], pk[0], 0x07060302), __builtin_amdgcn_perm(pk[3], pk[2], 0x07060302),
                                __builtin_amdgcn_perm(pk[5], pk[4], 0x07060302), __builtin_amdgcn_perm(pk[7], pk[6], 0x07060302)};
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
@@ -684,111 +690,139 @@ struct MxMatmul {
     void* y;                  // [M, N]
 };
 
-// A block of four waves owns 128 rows of B x 128 rows of A, a wave 64 x 64 of them (4 x 4 tiles of the scaled 16 x 16 x 128 instruction).  128 elements of K -- 64
-// bytes and four scale bytes a row -- go through LDS at a time, double-buffered, the next ones on their way in registers while these are multiplied: every
-// row is read once a block instead of twice.
+// A block of four waves owns BM rows of A x BN rows of B, a wave half of each (tiles of the scaled 16 x 16 x 128 instruction).  128 elements of K -- 64 bytes of codes and
+// four scale bytes a row -- go through LDS at a time, double-buffered, the next ones on their way in registers while these are multiplied.
+constexpr int MM_Q = 4;       // blocks of 32 a step
+template <int ROWS>
 struct MxTile {
-    uint4 codes[128][4];      // block q of row r at place mx_place(r, q): eight neighbouring lanes, which read eight rows' block q, meet eight different places modulo 128 bytes
-    unsigned scales[128];     // four blocks' bytes
+    u32x4 codes[ROWS][MM_Q];  // block q of row r at place mx_place(r, q): eight neighbouring lanes, which read eight rows' block q, meet eight different places modulo 128 bytes
+    unsigned scales[ROWS];    // four bytes
 };
 __device__ __forceinline__ int mx_place(int row, int q) { return q ^ ((row >> 1) & 3); }
 
-// a row's four scale bytes of blocks k .. k + 3 (behind the last block: scale 1)
-__device__ __forceinline__ unsigned mx_scales4(const uint8_t* row, int k, int Kb) {
-    if (k + 4 <= Kb) {                                            // (the same for the whole block of threads)
-        struct __attribute__((packed)) Bytes4 { unsigned v; };
-        return reinterpret_cast<const Bytes4*>(row + k)->v;
-    }
-    unsigned s = 0x7f7f7f7fu;
-    for (int b = 0; k + b < Kb; b++) s = (s & ~(0xffu << 8 * b)) | (unsigned)row[k + b] << 8 * b;
-    return s;
-}
-
-template <int DT>
+// WHOLE: K is a multiple of a step.  Otherwise every block behind the last is the last one's, with its codes masked to zero in B (as those behind K are, whatever the matrix
+// holds there) and scale 1, and a row's scales are read byte by byte.  Either way the loop has no branch: a branch around a load made the compiler wait for it there.
+template <int DT, int BM, int BN, bool WHOLE>
 __global__ __launch_bounds__(MX_T) void mx_matmul_kernel(const MxMatmul a, long long mtiles) {
-    __shared__ MxTile ta[2], tb[2];
-    const unsigned tid = threadIdx.x;
-    const int lane = tid & 63, wave = tid >> 6, col = lane & 15, q = lane >> 4;
-    const long long m0 = (blockIdx.x % mtiles) * 128, n0 = (blockIdx.x / mtiles) * 128;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    f32x4 acc[4][4];
+    constexpr int TM = BM / 32, TN = BN / 32, CA = BM / 64, CB = BN / 64;        // tiles a wave; rows a thread carries a block of
+    constexpr size_t OPERANDS = 2 * (sizeof(MxTile<BM>) + sizeof(MxTile<BN>)), RESULTS = sizeof(float) * 32 * (BN + 4);
+    static_assert(BM + BN <= MX_T, "a thread carries the scales of one row");
+    __shared__ __attribute__((aligned(16))) unsigned char lds[OPERANDS > RESULTS ? OPERANDS : RESULTS];
+    auto ta = reinterpret_cast<MxTile<BM>*>(lds);
+    auto tb = reinterpret_cast<MxTile<BN>*>(lds + 2 * sizeof(MxTile<BM>));
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, q = lane >> 4;
+    const long long m0 = (blockIdx.x % mtiles) * BM, n0 = (blockIdx.x / mtiles) * BN;
+    const int wm = (wave & 1) * (BM / 2), wn = (wave >> 1) * (BN / 2);
+    f32x4 acc[TN][TM];
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+    for (int t = 0; t < TN; t++)
 #pragma unroll
-        for (int u = 0; u < 4; u++) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // this thread's pieces of the tiles: block `blk` of rows tid / 4 and 64 further of A and of B, and the four scale bytes of a row of A (threads 0 .. 127) or of B.
+        for (int u = 0; u < TM; u++) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // this thread's pieces of the tiles: block `blk` of every 64th row from r0 on, and the four scale bytes of one row (of A: the first BM threads; of B: the last BN).
     // Rows behind the last are the last one's (their results are not stored).
     const int Kb = a.b.Kb, last = a.b.K & 31, r0 = tid >> 2, blk = tid & 3;
-    auto row_at = [](const MxMatrix& w, long long row) { return (size_t)min(row, w.rows - 1) * w.Kb; };
-    const uint4* const a0 = reinterpret_cast<const uint4*>(a.a.codes) + row_at(a.a, m0 + r0);
-    const uint4* const a1 = reinterpret_cast<const uint4*>(a.a.codes) + row_at(a.a, m0 + 64 + r0);
-    const uint4* const b0 = reinterpret_cast<const uint4*>(a.b.codes) + row_at(a.b, n0 + r0);
-    const uint4* const b1 = reinterpret_cast<const uint4*>(a.b.codes) + row_at(a.b, n0 + 64 + r0);
-    const uint8_t* const sr = tid < 128 ? a.a.scales + row_at(a.a, m0 + tid) : a.b.scales + row_at(a.b, n0 + tid - 128);
-    const int p0 = mx_place(r0, blk);                             // (the same place in row r0 + 64)
-    uint4 ca0, ca1, cb0, cb1;
+    const u32x4* const abase = reinterpret_cast<const u32x4*>(a.a.codes) + (size_t)m0 * Kb;
+    const u32x4* const bbase = reinterpret_cast<const u32x4*>(a.b.codes) + (size_t)n0 * Kb;
+    unsigned oa[CA], ob[CB];                                      // (inside a tile: at most 128 x 2^19 blocks)
+#pragma unroll
+    for (int h = 0; h < CA; h++) oa[h] = (unsigned)min((long long)(r0 + 64 * h), a.a.rows - 1 - m0) * Kb;
+#pragma unroll
+    for (int h = 0; h < CB; h++) ob[h] = (unsigned)min((long long)(r0 + 64 * h), a.b.rows - 1 - n0) * Kb;
+    const int srow = tid < BM ? tid : max(tid - (MX_T - BN), 0);
+    const uint8_t* const ps = tid < BM ? a.a.scales + (size_t)min(m0 + srow, a.a.rows - 1) * Kb : a.b.scales + (size_t)min(n0 + srow, a.b.rows - 1) * Kb;
+    unsigned* const stile = tid < BM ? ta[0].scales : tb[0].scales;
+    const int snext = (tid < BM ? sizeof(MxTile<BM>) : sizeof(MxTile<BN>)) / 4;
+    const int p0 = mx_place(r0, blk);                             // (the same place in rows 64 further)
+    u32x4 ca[CA], cb[CB];
     unsigned sc;
     auto fetch = [&](int k) {
-        const int at = min(k + blk, Kb - 1);
-        ca0 = a0[at];
-        ca1 = a1[at];
-        cb0 = b0[at];
-        cb1 = b1[at];
-        sc = mx_scales4(sr, k, Kb);
+        const unsigned at = WHOLE ? (unsigned)(k + blk) : (unsigned)min(k + blk, Kb - 1);
+#pragma unroll
+        for (int h = 0; h < CA; h++) ca[h] = abase[oa[h] + at];
+#pragma unroll
+        for (int h = 0; h < CB; h++) cb[h] = bbase[ob[h] + at];
+        if constexpr (WHOLE) {
+            struct __attribute__((packed)) Bytes4 { unsigned v; };
+            sc = reinterpret_cast<const Bytes4*>(ps + k)->v;
+        } else {
+            unsigned s[4];
+#pragma unroll
+            for (int b = 0; b < 4; b++) s[b] = ps[min(k + b, Kb - 1)];
+            sc = s[0] | s[1] << 8 | s[2] << 16 | s[3] << 24;
+        }
     };
     auto put = [&](int buf, int k) {
-        if (k + 4 >= Kb) {                                        // the last round: codes behind K are zero in one operand, whatever the matrix holds there
+        if constexpr (!WHOLE) {
             const int left = k + blk < Kb - 1 ? 32 : k + blk == Kb - 1 ? (last ? last : 32) : 0;
             unsigned mask[4];
 #pragma unroll
             for (int d = 0; d < 4; d++) mask[d] = left >= 8 * d + 8 ? ~0u : left <= 8 * d ? 0u : (1u << 4 * (left - 8 * d)) - 1u;
-            cb0.x &= mask[0]; cb0.y &= mask[1]; cb0.z &= mask[2]; cb0.w &= mask[3];
-            cb1.x &= mask[0]; cb1.y &= mask[1]; cb1.z &= mask[2]; cb1.w &= mask[3];
+#pragma unroll
+            for (int h = 0; h < CB; h++) { cb[h].x &= mask[0]; cb[h].y &= mask[1]; cb[h].z &= mask[2]; cb[h].w &= mask[3]; }
+            const int there = min(Kb - k, 4);                     // blocks of this step that exist; the others: scale 1
+            const unsigned keep = there >= 4 ? ~0u : (1u << 8 * there) - 1u;
+            sc = (sc & keep) | (0x7f7f7f7fu & ~keep);
         }
-        ta[buf].codes[r0][p0] = ca0;
-        ta[buf].codes[r0 + 64][p0] = ca1;
-        tb[buf].codes[r0][p0] = cb0;
-        tb[buf].codes[r0 + 64][p0] = cb1;
-        (tid < 128 ? ta : tb)[buf].scales[tid & 127] = sc;
+#pragma unroll
+        for (int h = 0; h < CA; h++) ta[buf].codes[r0 + 64 * h][p0] = ca[h];
+#pragma unroll
+        for (int h = 0; h < CB; h++) tb[buf].codes[r0 + 64 * h][p0] = cb[h];
+        if (BM + BN == MX_T || tid < BM || tid >= MX_T - BN) stile[buf * snext + srow] = sc;
+    };
+    auto multiply = [&](int buf) {
+        u32x4 bc[TN];
+        int bs[TN];
+#pragma unroll
+        for (int t = 0; t < TN; t++) {
+            const int r = wn + 16 * t + col;
+            bc[t] = tb[buf].codes[r][mx_place(r, q)];
+            bs[t] = (int)(tb[buf].scales[r] >> 8 * q);            // (the instruction takes the low byte)
+        }
+#pragma unroll
+        for (int u = 0; u < TM; u++) {
+            const int r = wm + 16 * u + col;
+            const u32x4 ac = ta[buf].codes[r][mx_place(r, q)];
+            const int as = (int)(ta[buf].scales[r] >> 8 * q);
+            const i32x8 y = {(int)ac.x, (int)ac.y, (int)ac.z, (int)ac.w, 0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < TN; t++) {
+                const i32x8 x = {(int)bc[t].x, (int)bc[t].y, (int)bc[t].z, (int)bc[t].w, 0, 0, 0, 0};
+                acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, acc[t][u], 4, 4, 0, bs[t], 0, as);
+            }
+        }
     };
     fetch(0);
     put(0, 0);
     __syncthreads();
-    for (int k = 0, buf = 0; k < Kb; k += 4, buf ^= 1) {
-        const bool more = k + 4 < Kb;
-        if (more) fetch(k + 4);
-        uint4 bc[4], ac[4];
-        int bs[4], as[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int rb = wn + 16 * t + col, ra = wm + 16 * t + col;
-            bc[t] = tb[buf].codes[rb][mx_place(rb, q)];
-            bs[t] = (int)(tb[buf].scales[rb] >> 8 * q);
-            ac[t] = ta[buf].codes[ra][mx_place(ra, q)];
-            as[t] = (int)(ta[buf].scales[ra] >> 8 * q);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const i32x8 x = {(int)bc[t].x, (int)bc[t].y, (int)bc[t].z, (int)bc[t].w, 0, 0, 0, 0};
-                const i32x8 y = {(int)ac[u].x, (int)ac[u].y, (int)ac[u].z, (int)ac[u].w, 0, 0, 0, 0};
-                acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, acc[t][u], 4, 4, 0, bs[t], 0, as[u]);     // (the low byte of the scale operands)
-            }
+    int buf = 0;
+    for (int k = MM_Q; k < Kb; k += MM_Q, buf ^= 1) {
+        fetch(k);
+        multiply(buf);
         __builtin_amdgcn_sched_barrier(0);     // (the loads are waited for here, behind the products, not in front of them)
-        if (more) put(buf ^ 1, k + 4);         // (the other buffer: its readers passed the barrier of the round before)
+        put(buf ^ 1, k);                       // (the other buffer: its readers passed the barrier of the round before)
         __syncthreads();
     }
-    float* tile = reinterpret_cast<float*>(ta);                   // 32 rows of 128 + 4 floats: half of the two buffers
-    static_assert(sizeof(float) * 32 * 132 <= sizeof(MxTile) * 2, "the results' tile fits the operands' buffers");
+    multiply(buf);
+    __syncthreads();
+    float* tile = reinterpret_cast<float*>(lds);
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < TM; u++) {
         if (u) __syncthreads();
 #pragma unroll
-        for (int t = 0; t < 4; t++) *reinterpret_cast<f32x4*>(tile + ((wave & 1) * 16 + col) * 132 + wn + 16 * t + 4 * q) = acc[t][u];
+        for (int t = 0; t < TN; t++) *reinterpret_cast<f32x4*>(tile + ((wave & 1) * 16 + col) * (BN + 4) + wn + 16 * t + 4 * q) = acc[t][u];
         __syncthreads();
-        mx_store_tile<DT, 32, 128>(tile, a.y, a.a.rows, a.b.rows, a.bias, a.relu, m0 + 16 * u, 64, n0);
+        mx_store_tile<DT, MX_T, 32, BN>(tile, a.y, a.a.rows, a.b.rows, a.bias, a.relu, m0 + 16 * u, BM / 2, n0);
     }
+}
+
+template <int DT, int BM, int BN>
+int mx_matmul_launch(const MxMatmul& a, hipStream_t st) {
+    const long long mtiles = (a.a.rows + BM - 1) / BM, tiles = mtiles * ((a.b.rows + BN - 1) / BN);
+    if (tiles >= (1ll << 31)) return VHAP_E_BADDIM;
+    if (a.b.K % (32 * MM_Q) == 0) mx_matmul_kernel<DT, BM, BN, true><<<(int)tiles, MX_T, 0, st>>>(a, mtiles);
+    else mx_matmul_kernel<DT, BM, BN, false><<<(int)tiles, MX_T, 0, st>>>(a, mtiles);
+    VHAP_LAUNCH_CHECK();
+    return VHAP_OK;
 }
 
 // ---- host side ----
@@ -961,9 +995,9 @@ extern "C" int vhap_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, 
     if (!a_codes || !a_scales || !b_codes || !b_scales || !y) return VHAP_E_NULLPTR;
     const int Kb = mx_kb(K);
     const MxMatmul a{{a_codes, a_scales, M, K, Kb}, {b_codes, b_scales, N, K, Kb}, bias, (call_flags & VHAP_CONV_OUT_RELU) ? 1 : 0, y};
-    const long long mtiles = (M + 127) / 128, tiles = mtiles * ((N + 127) / 128);
-    if (tiles >= (1ll << 31)) return VHAP_E_BADDIM;
-    MX_BY_TYPE(dtype, (mx_matmul_kernel<DT><<<(int)tiles, MX_T, 0, vhap_stream(stream)>>>(a, mtiles)));
-    VHAP_LAUNCH_CHECK();
-    return VHAP_OK;
+    // large tiles where they fill the chip, small ones where they would leave it empty
+    const bool large = ((M + 127) / 128) * ((N + 127) / 128) >= 256;
+    int rc = VHAP_OK;
+    MX_BY_TYPE(dtype, (rc = large ? mx_matmul_launch<DT, 128, 128>(a, vhap_stream(stream)) : mx_matmul_launch<DT, 64, 64>(a, vhap_stream(stream))));
+    return rc;
 }
