@@ -697,6 +697,13 @@ int vhap_tex_pca_fwd(const float* mean, const float* basis, const float* code, i
                      float* term_accum, vhap_stream_t stream);
 int vhap_tex_pca_bwd(const float* basis, const float* src, const float* d_base, const float* code, int n, int S, int T, float s_reg,
                      const float* d_term, float* g_work, float* d_code, vhap_stream_t stream);
+/*   mx4: the same with the basis in microscaled 4-bit floats (codes [S*S*3, 16 ceil(n / 32)], scales [S*S*3, ceil(n / 32)]: vhap_mx4_quantize of [S*S*3, n]); n <= 4096; d_code
+ *        is a sum in a fixed order there; workspace: _bwd_workspace_bytes, in use until the call's launches are done. */
+int vhap_tex_pca_mx4_fwd(const float* mean, const uint8_t* codes, const uint8_t* scales, const float* code, int n, int S, int T, float s_reg, float* src,
+                         float* base, float* term_accum, vhap_stream_t stream);
+size_t vhap_tex_pca_mx4_bwd_workspace_bytes(int n, int S);
+int vhap_tex_pca_mx4_bwd(const uint8_t* codes, const uint8_t* scales, const float* src, const float* d_base, const float* code, int n, int S, int T,
+                         float s_reg, const float* d_term, float* g_work, void* workspace, size_t workspace_bytes, float* d_code, vhap_stream_t stream);
 int vhap_adam_step(int n_tensors, float* const* params, const float* const* grads, float* const* exp_avg,
                    float* const* exp_avg_sq, const int64_t* numel, const int32_t* lr_index,
                    const float* lr_device, int32_t* step_device, float beta1, float beta2, float eps,

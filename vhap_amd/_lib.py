@@ -111,6 +111,9 @@ SIGNATURES = {
     "vhap_tex_prep_bwd_adam_base": (c_i, [c_fp] * 5 + [c_i, c_fp, c_i, c_f, c_f] + [c_fp] * 5 + [c_f, c_f, c_f, c_fp, c_i, c_fp]),
     "vhap_tex_pca_fwd": (c_i, [c_fp] * 3 + [c_i, c_i, c_i, c_f] + [c_fp] * 4),
     "vhap_tex_pca_bwd": (c_i, [c_fp] * 4 + [c_i, c_i, c_i, c_f] + [c_fp] * 4),
+    "vhap_tex_pca_mx4_fwd": (c_i, [c_fp] * 4 + [c_i, c_i, c_i, c_f] + [c_fp] * 4),
+    "vhap_tex_pca_mx4_bwd_workspace_bytes": (c_sz, [c_i, c_i]),
+    "vhap_tex_pca_mx4_bwd": (c_i, [c_fp] * 5 + [c_i, c_i, c_i, c_f] + [c_fp] * 3 + [c_sz] + [c_fp] * 2),
     "vhap_tex_prep_bwd_adam_rows": (c_i, [c_fp] * 5 + [c_i, c_i, c_i, c_f, c_f] + [c_fp] * 5 + [c_f, c_f, c_f, c_i, c_fp]),
     "vhap_tex_carry_halo_floats": (c_sz, [c_i]),
     "vhap_tex_carry_prime": (c_i, [c_fp] * 3 + [c_i, c_f, c_f] + [c_fp] * 5),

@@ -35,6 +35,7 @@ class ModelConfig(Config):                                              # base.p
     remove_lip_inside: bool = False
     tex_resolution: int = 2048
     tex_painted: bool = True
+    tex_basis_format: str = "fp32"      # of the PCA texture space (tex_painted = False): "mxfp4" holds its basis in 4.25 bits an element (not in the reference)
     tex_extra: bool = True
     tex_clusters: Tuple[str, ...] = ("skin", "hair", "boundary", "lips_tight", "teeth", "sclerae", "irises")
     residual_tex: bool = True
@@ -62,6 +63,7 @@ class LearningRateConfig(Config):                                       # base.p
     dynamic_offset: float = 5e-4
     camera: float = 5e-3
     light: float = 5e-3
+    max_grad_norm: Optional[float] = None   # clip the step's gradients to this global 2-norm (not in the reference)
 
 
 @dataclass

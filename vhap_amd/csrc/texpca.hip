@@ -6,6 +6,7 @@
 // vhap_tex_prep_fwd.  HBM-bound: the basis is [S*S*3, n] floats = 315 MB at n = 100, read once forward and once backward:
 //   forward : one WAVE per row of the basis (lanes over the n coefficients, 400 contiguous bytes per row, DPP sum), four rows in flight;
 //             then one thread per texel of the T x T base (nearest source texel, channel swap, / 255, clamp)
+//   (vhap_tex_pca_mx4_*: the basis in microscaled 4-bit floats, 42 MB: the rows and d(code) are the 4-bit linear and its input's gradient, mx.hip)
 //   backward: per source texel the sum of d(base) over the texels it was copied to, masked by the clamp; then d(code) = basis^T g with
 //             one wave per run of rows, two coefficients per lane in registers, one atomic per coefficient and wave.
 #include "common.h"
@@ -66,9 +67,13 @@ __global__ __launch_bounds__(256) void tex_pca_resize_kernel(const float* __rest
     }
 }
 
+// (reg != null: block 0 also adds the regulariser's gradient 2 s_reg code d_term to reg[n])
 // g[r] (source texel, source channel) = 1/255 * [0 <= src/255 <= 1] * sum over the base texels copied from it of d_base
 __global__ __launch_bounds__(256) void tex_pca_gather_kernel(const float* __restrict__ src, const float* __restrict__ d_base, int S, int T, float scale,
-                                                             float* __restrict__ g) {
+                                                             float* __restrict__ g, const float* __restrict__ code = nullptr, int n = 0, float s_reg = 0.f,
+                                                             const float* __restrict__ d_term = nullptr, float* __restrict__ reg = nullptr) {
+    if (reg && blockIdx.x == 0 && blockIdx.y == 0)
+        for (int k = threadIdx.x; k < n; k += 256) reg[k] += 2.0f * s_reg * code[k] * (d_term ? d_term[0] : 1.0f);
     const int sx = blockIdx.x * 256 + threadIdx.x, sy = blockIdx.y;
     if (sx >= S) return;
     // the base texels whose nearest source is (sy, sx): a contiguous run per axis -- found by stepping from the estimate
@@ -155,4 +160,34 @@ extern "C" int vhap_tex_pca_bwd(const float* basis, const float* src, const floa
     tex_pca_code_bwd_kernel<<<vhap_cdiv(R, 4 * rows_per_wave), 256, 0, st>>>(basis, g_work, n, R, rows_per_wave, code, s_reg, d_term, d_code);
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
+}
+
+extern "C" int vhap_tex_pca_mx4_fwd(const float* mean, const uint8_t* codes, const uint8_t* scales, const float* code, int n, int S, int T, float s_reg,
+                                    float* src, float* base, float* term_accum, vhap_stream_t stream) {
+    VHAP_ENTER();
+    if (!mean || !codes || !scales || !code || !src || !base) return VHAP_E_NULLPTR;
+    if (n <= 0 || n > 4096 || S <= 0 || T <= 0 || S > 8192 || T > 16384) return VHAP_E_BADDIM;
+    const int rc = vhap_mx4_linear(code, VHAP_DTYPE_F32, n, 1, codes, scales, 3ll * S * S, n, mean, src, stream);
+    if (rc != VHAP_OK) return rc;
+    tex_pca_resize_kernel<<<dim3(vhap_cdiv(T, 256), T), 256, 0, vhap_stream(stream)>>>(src, S, T, (float)S / (float)T, base, code, n, s_reg, term_accum);
+    VHAP_LAUNCH_CHECK();
+    return VHAP_OK;
+}
+
+extern "C" size_t vhap_tex_pca_mx4_bwd_workspace_bytes(int n, int S) {
+    return n <= 0 || S <= 0 ? 0 : vhap_mx4_linear_input_grad_workspace_bytes(1, 3ll * S * S, n);
+}
+
+extern "C" int vhap_tex_pca_mx4_bwd(const uint8_t* codes, const uint8_t* scales, const float* src, const float* d_base, const float* code, int n, int S, int T,
+                                    float s_reg, const float* d_term, float* g_work, void* workspace, size_t workspace_bytes, float* d_code,
+                                    vhap_stream_t stream) {
+    VHAP_ENTER();
+    if (!codes || !scales || !src || !d_base || !code || !g_work || !workspace || !d_code) return VHAP_E_NULLPTR;
+    if (n <= 0 || n > 4096 || S <= 0 || T <= 0 || S > 8192 || T > 16384) return VHAP_E_BADDIM;
+    if (workspace_bytes < vhap_tex_pca_mx4_bwd_workspace_bytes(n, S)) return VHAP_E_WORKSPACE;
+    tex_pca_gather_kernel<<<dim3(vhap_cdiv(S, 256), S), 256, 0, vhap_stream(stream)>>>(src, d_base, S, T, (float)S / (float)T, g_work, code, n, s_reg, d_term,
+                                                                                       s_reg != 0.f ? d_code : nullptr);
+    VHAP_LAUNCH_CHECK();
+    return vhap_mx4_linear_input_grad(g_work, VHAP_DTYPE_F32, 3ll * S * S, 1, codes, scales, 3ll * S * S, n, workspace, workspace_bytes, d_code,
+                                      VHAP_CALL_MX_ACCUMULATE, stream);
 }

@@ -20,7 +20,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .landmarks import _chk, _Conv
+from .landmarks import _chk, _Conv, new_conv
 from .ops import _p, _stream
 
 TRUNK = (("conv1_1", "conv1_2"), ("conv2_1", "conv2_2"), ("conv3_1", "conv3_2", "conv3_3"), ("conv4_1", "conv4_2", "conv4_3"),
@@ -38,14 +38,15 @@ def _maxpool2(x):
 
 class S3FD:
     """The network of oracle/sfd_ref.py::S3FD from the package's state dict.  forward(x [N,H,W,3] float32 on the GPU: BGR minus the means, channel
-    last) -> list of six (cls [N,h,w,ncls], loc [N,h,w,4]) pairs, channel-last views of the heads' 8-channel outputs."""
+    last) -> list of six (cls [N,h,w,ncls], loc [N,h,w,4]) pairs, channel-last views of the heads' 8-channel outputs.  `pointwise`: "fp32", or "mxfp4": fc7,
+    conv6_1 and conv7_1 as products of microscaled 4-bit matrices (as in landmarks.FAN2D)."""
 
-    def __init__(self, state_dict, device="cuda"):
+    def __init__(self, state_dict, device="cuda", pointwise="fp32"):
         if not str(device).startswith("cuda"):
             raise RuntimeError("S3FD runs on the HIP device only (there is no CPU path)")
         sd = {k[7:] if k.startswith("module.") else k: v for k, v in state_dict.items()}
         self.device = device
-        c = lambda name, **kw: _Conv(sd[name + ".weight"], sd[name + ".bias"], out_relu=True, device=device, **kw)
+        c = lambda name, **kw: _Conv(sd[name + ".weight"], sd[name + ".bias"], out_relu=True, device=device, pointwise=pointwise, **kw)
         self.trunk = [[c(n, pad=1) for n in stage] for stage in TRUNK]
         self.fc6, self.fc7 = c("fc6", pad=3), c("fc7")
         self.conv6_1, self.conv6_2 = c("conv6_1"), c("conv6_2", stride=2, pad=1)
@@ -62,9 +63,7 @@ class S3FD:
 
     @staticmethod
     def _run(conv, x):
-        N, H, W, _ = x.shape
-        Ho, Wo = (H + 2 * conv.pad - conv.KH) // conv.stride + 1, (W + 2 * conv.pad - conv.KW) // conv.stride + 1
-        return conv(x, 0, conv.cin, torch.empty(N, Ho, Wo, conv.cout, dtype=torch.float32, device=x.device), 0)
+        return new_conv(conv, x)
 
     def __call__(self, x):
         if not (isinstance(x, torch.Tensor) and x.is_cuda):
@@ -129,13 +128,13 @@ def nms(dets, thresh=0.3):
 
 class SFDDetector:
     """`face_alignment`'s SFDDetector.detect_from_image over S3FD: callable(img [H,W,3] uint8 RGB) -> list of [x1, y1, x2, y2, score] arrays.
-    `weights`: the package's state dict, or a path torch.load can read."""
+    `weights`: the package's state dict, or a path torch.load can read.  `pointwise`: S3FD."""
 
-    def __init__(self, weights, device="cuda", filter_threshold=0.5, pre_threshold=0.05, nms_threshold=0.3):
+    def __init__(self, weights, device="cuda", filter_threshold=0.5, pre_threshold=0.05, nms_threshold=0.3, pointwise="fp32"):
         if isinstance(weights, (str, os.PathLike)):
             weights = torch.load(weights, map_location="cpu")
             weights = weights.get("state_dict", weights) if isinstance(weights, dict) else weights.state_dict()
-        self.net = S3FD(weights, device=device)
+        self.net = S3FD(weights, device=device, pointwise=pointwise)
         self.device, self.filter_threshold, self.pre_threshold, self.nms_threshold = device, filter_threshold, pre_threshold, nms_threshold
 
     def candidates(self, img):

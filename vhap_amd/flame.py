@@ -11,6 +11,7 @@ import torch
 import torch.nn as nn
 
 from . import lbs as L
+from . import mx
 from . import fused as FU
 from .topology import FlameTopology
 
@@ -166,9 +167,12 @@ class FlameTexPCA(nn.Module):
     """flame.py:665-688 -- the FLAME PCA texture space (`tex_painted = False`): texture = mean + basis . code on a 512 x 512 x 3 grid in
     0..255, B G R; forward(texcode [B, n]) -> [B, 3, T, T]: nearest resize to the working resolution, channels to R G B, / 255, clamp.
     `tex_space`: a path to FLAME_texture.npz (`mean`, `tex_dir`) or a mapping with those two arrays (tests: a synthetic space of the same
-    layout -- the licensed file is not in this container)."""
+    layout -- the licensed file is not in this container).  `basis_format`: "fp32", or "mxfp4": the basis in microscaled 4-bit floats
+    (vhap_amd.mx: blocks of 32 coefficients; 42 instead of 315 MB at 100 coefficients, read twice a step).  A coefficient is then off by
+    at most a quarter of itself or a sixteenth of the largest of its 32, whichever is more: the SPACE is another one, close to the one given; texture and
+    gradient are computed in it as exactly as in fp32."""
 
-    def __init__(self, tex_params, tex_size=512, tex_space=None):
+    def __init__(self, tex_params, tex_size=512, tex_space=None, basis_format="fp32"):
         super().__init__()
         self.tex_size = int(tex_size)
         space = np.load(tex_space) if isinstance(tex_space, (str, bytes)) or hasattr(tex_space, "__fspath__") else tex_space
@@ -178,11 +182,29 @@ class FlameTexPCA(nn.Module):
         self.src_size = int(round((mean.shape[1] // 3) ** 0.5))
         assert self.src_size * self.src_size * 3 == mean.shape[1] == basis.shape[0]
         self.register_buffer("texture_mean", torch.from_numpy(mean)[None, ...])                           # [1, 1, S*S*3]
-        self.register_buffer("texture_basis", torch.from_numpy(np.ascontiguousarray(basis))[None, ...])   # [1, S*S*3, n]
+        self.basis_format = basis_format
+        basis = torch.from_numpy(np.ascontiguousarray(basis))
+        if basis_format == "fp32":
+            self.register_buffer("texture_basis", basis[None, ...])                                       # [1, S*S*3, n]
+        elif basis_format == "mxfp4":
+            q = mx.quantize_host(basis)
+            self.register_buffer("basis_codes", q.codes)                                                  # [S*S*3, 16 ceil(n / 32)]
+            self.register_buffer("basis_scales", q.scales)
+        else:
+            raise ValueError(f"basis_format 'fp32' or 'mxfp4', got {basis_format!r}")
+        self.n_params = int(basis.shape[1])
+
+    def mx_basis(self):
+        return mx.MXTensor(self.basis_codes, self.basis_scales, (self.basis_codes.shape[0], self.n_params))
 
     def forward(self, texcode):
         S = self.src_size
-        texture = self.texture_mean + (self.texture_basis * texcode[:, None, :]).sum(-1)
+        if self.basis_format == "fp32":
+            texture = self.texture_mean + (self.texture_basis * texcode[:, None, :]).sum(-1)
+        elif texcode.is_cuda:
+            texture = mx.linear(texcode, self.mx_basis(), self.texture_mean.reshape(-1))
+        else:
+            texture = self.texture_mean.reshape(1, -1) + texcode @ self.mx_basis().dequantize(torch.float32).to(texcode.dtype).t()
         texture = texture.reshape(texcode.shape[0], S, S, 3).permute(0, 3, 1, 2)
         texture = torch.nn.functional.interpolate(texture, [self.tex_size, self.tex_size])
         texture = texture[:, [2, 1, 0], :, :]

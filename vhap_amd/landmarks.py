@@ -26,7 +26,7 @@ import os
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, mx
 from .ops import _p, _stream
 
 # mirror pairs of the 68-point markup (the package's flip(..., is_label=True) swaps them when it averages the flipped pass)
@@ -59,7 +59,7 @@ def _workspace(device):
 class _Conv:
     """one convolution's device-side constants: weight [KH,KW,Cin,Cout], optional bias, optional input BatchNorm as (scale, shift)"""
 
-    def __init__(self, w, bias=None, bn_in=None, bn_out=None, stride=1, pad=0, in_relu=False, out_relu=False, device="cuda"):
+    def __init__(self, w, bias=None, bn_in=None, bn_out=None, stride=1, pad=0, in_relu=False, out_relu=False, device="cuda", pointwise="fp32"):
         w = w.detach().to(torch.float32)
         cout = w.shape[0]
         b = None if bias is None else bias.detach().to(torch.float32).clone()
@@ -73,6 +73,12 @@ class _Conv:
         self.KH, self.KW, self.cin, self.cout = int(w.shape[2]), int(w.shape[3]), int(w.shape[1]), int(cout)
         self.stride, self.pad = int(stride), int(pad)
         self.flags = (_lib.CONV_IN_RELU if in_relu else 0) | (_lib.CONV_OUT_RELU if out_relu else 0)
+        # pointwise="mxfp4": a 1 x 1 convolution as a product of 4-bit matrices (weights once, activations at every call)
+        if pointwise not in ("fp32", "mxfp4"):
+            raise ValueError(f"pointwise 'fp32' or 'mxfp4', got {pointwise!r}")
+        self.mx_w, self.out_relu = None, bool(out_relu)
+        if pointwise == "mxfp4" and self.KH == self.KW == self.stride == 1 and self.pad == 0 and bn_in is None and not in_relu:
+            self.mx_w = mx.quantize(self.w.view(self.cin, self.cout).t().contiguous())
 
     def __call__(self, x, x_off, x_cin, out, out_off, accumulate=False):
         """x, out: NHWC buffers; the convolution reads channels [x_off, x_off + cin) of x and writes [out_off, out_off + cout) of out"""
@@ -84,6 +90,15 @@ class _Conv:
                                             _p(ws), ws.numel(), self.flags | (_lib.CONV_ACCUMULATE if accumulate else 0), _stream())
         _chk(rc, "vhap_conv2d_nhwc_ws")
         return out
+
+
+def new_conv(conv, x):
+    """`conv` over all channels of x [N,H,W,C] into a new buffer"""
+    N, H, W, C = x.shape
+    if conv.mx_w is not None:
+        return mx.matmul(mx.quantize(x.view(-1, C)), conv.mx_w, conv.bias, relu=conv.out_relu).view(N, H, W, conv.cout)
+    Ho, Wo = (H + 2 * conv.pad - conv.KH) // conv.stride + 1, (W + 2 * conv.pad - conv.KW) // conv.stride + 1
+    return conv(x, 0, C, torch.empty(N, Ho, Wo, conv.cout, dtype=torch.float32, device=x.device), 0)
 
 
 def _bn(sd, prefix, eps=1e-5):
@@ -127,9 +142,11 @@ def _avgpool2(x):
 
 class FAN2D:
     """The network of oracle/fan_ref.py::FAN from the package's state dict.  forward(x [N,3,256,256] float32 on the GPU, RGB in [0, 1]) ->
-    list of `num_modules` heat-map tensors [N,68,64,64] (channel-first VIEWS of the channel-last buffers the kernels write)."""
+    list of `num_modules` heat-map tensors [N,68,64,64] (channel-first VIEWS of the channel-last buffers the kernels write).
+    `pointwise`: "fp32", or "mxfp4": the 1 x 1 convolutions behind the hourglasses as products of microscaled 4-bit matrices (vhap_amd.mx; weights and
+    activations rounded to 4 bits in blocks of 32 channels: approximate, to be checked on the weights in use)."""
 
-    def __init__(self, state_dict, num_modules=4, n_landmarks=68, device="cuda"):
+    def __init__(self, state_dict, num_modules=4, n_landmarks=68, device="cuda", pointwise="fp32"):
         if not str(device).startswith("cuda"):
             raise RuntimeError("FAN2D runs on the HIP device only (there is no CPU path)")
         sd = {k[7:] if k.startswith("module.") else k: v for k, v in state_dict.items()}
@@ -145,11 +162,11 @@ class FAN2D:
             blocks["b2_plus_1"] = _Block(sd, f"m{i}.b2_plus_1", 256, 256, device)
             self.hg.append(blocks)
             self.top.append(_Block(sd, f"top_m_{i}", 256, 256, device))
-            self.last.append(_Conv(sd[f"conv_last{i}.weight"], sd[f"conv_last{i}.bias"], bn_out=_bn(sd, f"bn_end{i}"), out_relu=True, device=device))
-            self.l.append(_Conv(sd[f"l{i}.weight"], sd[f"l{i}.bias"], device=device))
+            self.last.append(_Conv(sd[f"conv_last{i}.weight"], sd[f"conv_last{i}.bias"], bn_out=_bn(sd, f"bn_end{i}"), out_relu=True, device=device, pointwise=pointwise))
+            self.l.append(_Conv(sd[f"l{i}.weight"], sd[f"l{i}.bias"], device=device, pointwise=pointwise))
             if i < self.num_modules - 1:
-                self.bl.append(_Conv(sd[f"bl{i}.weight"], sd[f"bl{i}.bias"], device=device))
-                self.al.append(_Conv(sd[f"al{i}.weight"], sd[f"al{i}.bias"], device=device))
+                self.bl.append(_Conv(sd[f"bl{i}.weight"], sd[f"bl{i}.bias"], device=device, pointwise=pointwise))
+                self.al.append(_Conv(sd[f"al{i}.weight"], sd[f"al{i}.bias"], device=device, pointwise=pointwise))
 
     def _hourglass(self, B, level, x):
         up1 = B[f"b1_{level}"](x)
@@ -162,9 +179,7 @@ class FAN2D:
         return out
 
     def _conv_new(self, conv, x):
-        N, H, W, C = x.shape
-        Ho, Wo = (H + 2 * conv.pad - conv.KH) // conv.stride + 1, (W + 2 * conv.pad - conv.KW) // conv.stride + 1
-        return conv(x, 0, C, torch.empty(N, Ho, Wo, conv.cout, dtype=torch.float32, device=x.device), 0)
+        return new_conv(conv, x)
 
     @torch.no_grad()
     def forward(self, x):
@@ -255,13 +270,13 @@ def heatmaps_to_points(hm, center=None, scale=None):
 class LandmarkDetectorFA:
     """vhap/util/landmark_detector_fa.py:25-78 over FAN2D.  `weights`: the package's state dict, or a path torch.load can read.
     `face_detector`: callable(img [H,W,3] uint8) -> list of (x1, y1, x2, y2, score); None: the whole frame is the box (the package's `sfd`
-    detector is a second third-party network, not built)."""
+    detector is a second third-party network, not built).  `pointwise`: FAN2D."""
 
-    def __init__(self, weights, face_detector=None, flip_input=True, device="cuda", num_modules=4):
+    def __init__(self, weights, face_detector=None, flip_input=True, device="cuda", num_modules=4, pointwise="fp32"):
         if isinstance(weights, (str, os.PathLike)):
             weights = torch.load(weights, map_location="cpu")
             weights = weights.get("state_dict", weights) if isinstance(weights, dict) else weights.state_dict()
-        self.net = FAN2D(weights, num_modules=num_modules, device=device)
+        self.net = FAN2D(weights, num_modules=num_modules, device=device, pointwise=pointwise)
         self.face_detector, self.flip_input, self.device = face_detector, bool(flip_input), device
 
     def landmarks_from_boxes(self, imgs, boxes):

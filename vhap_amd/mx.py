@@ -12,7 +12,7 @@ What it is for here: the linear spaces a fit reads whole in every step and never
 (FlameTexPCA(basis_format="mxfp4")) -- and the pointwise convolutions of the landmark networks (pointwise="mxfp4").
 
 All calls enqueue on the current stream of the tensors' device, allocate what they need through torch, and never synchronise.  No CPU path: CPU tensors raise
-(MXTensor.dequantize excepted, which also runs on the CPU, in torch operations, for checks and for host-side models)."""
+(excepted: MXTensor.dequantize, which also runs on the CPU, and quantize_host, which only does, both in torch operations: for models built on the host)."""
 import torch
 
 from . import _lib
@@ -91,6 +91,31 @@ def quantize(x):
     """x [..., K] -> MXTensor of the same shape: blocks of 32 along the last axis.  The scale is the power of two that puts a block's largest magnitude into
     [4, 8); codes are the nearest ones, halves to the even code, magnitudes above 6 become 6.  A block with a NaN or an infinity becomes NaN as a whole."""
     return MXTensor._of(*_lib.host().quantize(x), x.shape)
+
+
+def quantize_host(x):
+    """quantize of a CPU tensor, in torch operations, to the same codes and scales (a model's constants are laid out once, before they move to the device)"""
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"quantize_host: a float32, bfloat16 or float16 tensor, got {x.dtype}")
+    if x.is_cuda or x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize_host: a CPU tensor with at least one element along the last axis, got {tuple(x.shape)} on {x.device}")
+    K = x.shape[-1]
+    v = torch.nn.functional.pad(x.detach().float().reshape(-1, K), (0, -K % BLOCK)).view(-1, -(-K // BLOCK), BLOCK)
+    bits = v.view(torch.int32) & 0x7fffffff
+    field = bits.amax(-1) >> 23                                            # the largest exponent field; 255: a NaN or an infinity is among them
+    byte = torch.where(field == 255, field, (field - 2).clamp(min=0))
+    # x / 2^(byte - 127) without leaving fp32 (exact: powers of two built from their bits; byte 0 in two steps of 2^64 and 2^63)
+    up = torch.where(byte == 0, torch.full_like(byte, 127 + 64), torch.full_like(byte, 127))
+    rest = torch.where(byte == 0, torch.full_like(byte, 127 + 63), (254 - byte).clamp(min=1))
+    s = v.abs() * (up << 23).view(torch.float32)[..., None] * (rest << 23).view(torch.float32)[..., None]
+    step = torch.where(s < 2, 0.5, torch.where(s < 4, 1.0, 2.0))
+    q = (torch.round(s / step) * step).clamp(max=6.0)                       # halves to even
+    code = torch.where(q < 2, 2 * q, torch.where(q < 4, q + 2, q / 2 + 4))  # 0, .5, 1, 1.5 | 2, 3 | 4, 6 -> 0 .. 7
+    code = torch.nan_to_num(code, nan=0.0).to(torch.uint8) | (torch.signbit(v).to(torch.uint8) << 3)
+    code[byte == 255] = 0
+    code = code.reshape(v.shape[0], -1)
+    kb = -(-K // BLOCK)
+    return MXTensor((code[:, 0::2] | code[:, 1::2] << 4).contiguous().view(x.shape[:-1] + (16 * kb,)), byte.to(torch.uint8).view(x.shape[:-1] + (kb,)).contiguous(), x.shape)
 
 
 def linear(x, w, bias=None):

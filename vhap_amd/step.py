@@ -134,7 +134,11 @@ class NativeStep:
                 raise NotImplementedError("the PCA texture model at a resolution other than tex_resolution")
             S, n = self.pca.src_size, int(tr.tex_pca.shape[0])
             self.pca_mean = self.pca.texture_mean.reshape(-1).contiguous()
-            self.pca_basis = self.pca.texture_basis[0].contiguous()              # [S*S*3, n]
+            self.pca_mx = self.pca.mx_basis() if self.pca.basis_format == "mxfp4" else None
+            if self.pca_mx is None:
+                self.pca_basis = self.pca.texture_basis[0].contiguous()          # [S*S*3, n]
+            else:
+                self.pca_ws = E(max(1, self.L.vhap_tex_pca_mx4_bwd_workspace_bytes(n, S) // 4))
             self.pca_src, self.pca_work = E(S * S * 3), E(S * S * 3)
             self.pca_train = tex_on
             self.pca_scale = float((w.reg_tex_pca if tex_on else None) or 0.0) / n
@@ -405,7 +409,10 @@ class NativeStep:
         `ready()` is called behind the pyramid -- what the rasteriser waits for -- ahead of the offset regularisers."""
         L, tr, T, acc = self.L, self.tr, self.T, self.accF
         st = _stream()
-        if self.pca is not None and self.tex_fwd_on:
+        if self.pca is not None and self.tex_fwd_on and self.pca_mx is not None:
+            _chk(L.vhap_tex_pca_mx4_fwd(_p(self.pca_mean), _p(self.pca_mx.codes), _p(self.pca_mx.scales), _p(tr.tex_pca), int(tr.tex_pca.shape[0]), self.pca.src_size, T,
+                                        self.pca_scale, _p(self.pca_src), _p(self.painted), _p(acc[9:10]), st), "vhap_tex_pca_mx4_fwd")
+        elif self.pca is not None and self.tex_fwd_on:
             _chk(L.vhap_tex_pca_fwd(_p(self.pca_mean), _p(self.pca_basis), _p(tr.tex_pca), int(tr.tex_pca.shape[0]), self.pca.src_size, T,
                                     self.pca_scale, _p(self.pca_src), _p(self.painted), _p(acc[9:10]), st), "vhap_tex_pca_fwd")
         if self.carry:
@@ -778,7 +785,11 @@ class NativeStep:
         d_base = _p(self.d_base) if self.pca is not None else 0       # (PCA texture model: d(base texture) comes out of the same pass)
 
         def pca_bwd():
-            if self.pca is not None:
+            if self.pca is not None and self.pca_mx is not None:
+                _chk(L.vhap_tex_pca_mx4_bwd(_p(self.pca_mx.codes), _p(self.pca_mx.scales), _p(self.pca_src), _p(self.d_base), _p(tr.tex_pca), int(tr.tex_pca.shape[0]),
+                                            self.pca.src_size, T, self.pca_scale, _p(self.ones), _p(self.pca_work), _p(self.pca_ws), self.pca_ws.numel() * 4,
+                                            _p(g["tex_pca"]), _stream()), "vhap_tex_pca_mx4_bwd")
+            elif self.pca is not None:
                 _chk(L.vhap_tex_pca_bwd(_p(self.pca_basis), _p(self.pca_src), _p(self.d_base), _p(tr.tex_pca), int(tr.tex_pca.shape[0]),
                                         self.pca.src_size, T, self.pca_scale, _p(self.ones), _p(self.pca_work), _p(g["tex_pca"]), _stream()),
                      "vhap_tex_pca_bwd")

@@ -69,6 +69,9 @@ def main(argv=None):
                     "(tracker.py:1263-1277; landmark_source 'face-alignment'), on the matrix cores (vhap_amd.landmarks)")
     ap.add_argument("--face-detector-weights", default=None, help="state dict of the package's `sfd` face detector (S3FD on the matrix cores, "
                     "vhap_amd.face_detector); without it the whole frame is the face box")
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="clip every step's gradients to this global 2-norm (cfg.lr.max_grad_norm; not in the reference)")
+    ap.add_argument("--tex-basis-format", choices=("fp32", "mxfp4"), default=None, help="how the PCA texture basis is held on the device (cfg.model.tex_basis_format; "
+                    "not in the reference)")
     ap.add_argument("--dry-run", action="store_true", help="load + convert the configuration, print the stage plan, do not open data or fit")
     ap.add_argument("-h", "--help", action="store_true")
     a, rest = ap.parse_known_args(argv)
@@ -91,6 +94,10 @@ def main(argv=None):
         cfg.exp.output_folder = Path(a.output_folder)
     if a.device is not None:
         cfg.device = a.device
+    if a.max_grad_norm is not None:
+        cfg.lr.max_grad_norm = a.max_grad_norm                       # (fields of this side: convert_config reads them by name)
+    if a.tex_basis_format is not None:
+        cfg.model.tex_basis_format = a.tex_basis_format
     from .reference_adapter import convert_config
     mine = convert_config(cfg)
     stages = ["lmk_init_rigid", "lmk_init_all"] + (["rgb_init_texture", "rgb_init_all"] + (["rgb_init_offset"] if mine.model.use_static_offset else [])

@@ -44,7 +44,8 @@ class FlameTracker:
         if cfg.model.tex_painted:
             self.flame_tex_painted = FlameTexPainted(base_texture).to(self.device)
         else:
-            self.flame_tex_pca = FlameTexPCA(cfg.model.n_tex, tex_size=cfg.model.tex_resolution, tex_space=base_texture).to(self.device)
+            self.flame_tex_pca = FlameTexPCA(cfg.model.n_tex, tex_size=cfg.model.tex_resolution, tex_space=base_texture,
+                                             basis_format=cfg.model.tex_basis_format).to(self.device)
             self.flame_tex_painted = lambda: self.flame_tex_pca(self.tex_pca[None, :]).detach()     # (read-only views of the current base texture)
         self.flame_uvmask = FlameUvMask(topo).to(self.device)
         if cfg.render.backend != "hip":
@@ -113,7 +114,7 @@ class FlameTracker:
         groups.append({"params": rest})
         on_gpu = str(self.device).startswith("cuda")
         if on_gpu and self.fused and self.native:
-            return NV.HipAdam(groups, lr=lr.base * lr_scale)        # one launch for all parameter tensors
+            return NV.HipAdam(groups, lr=lr.base * lr_scale, max_grad_norm=lr.max_grad_norm)        # one launch for all parameter tensors
         return torch.optim.Adam(groups, lr=lr.base * lr_scale, capturable=on_gpu)   # device step counter: graph-capturable
 
     # ---- model ----
@@ -918,9 +919,18 @@ class GlobalTracker(FlameTracker):
         E_total.backward()
         if self.dist is not None:
             self.dist.average_gradients([p for g in optimizer.param_groups for p in g["params"]])
+        self.clip_gradients(optimizer)
         optimizer.step()
         self.global_step += 1
         return log_dict
+
+    def clip_gradients(self, optimizer):
+        """cfg.lr.max_grad_norm for an optimiser that does not clip by itself (HipAdam does, inside its update)"""
+        limit = self.cfg.lr.max_grad_norm
+        if limit is None or isinstance(optimizer, NV.HipAdam):
+            return
+        params = [p for g in optimizer.param_groups for p in g["params"]]
+        (NV.clip_grad_norm_ if str(self.device).startswith("cuda") else torch.nn.utils.clip_grad_norm_)(params, float(limit))
 
     def initialize_next_timtestep(self, timesteps):
         """tracker.py:1515-1529 (including its skip of the last frame)."""
@@ -1375,7 +1385,8 @@ class GraphedStep:
                 # the step counter is advanced at the head of the step (side branch), so that no piece of the update has to be last
                 tex = tracker.tex_extra
                 split = tex is not None and any(p is tex for p in self.params) and len(self.params) > 1 and ns.tex_bwd_on and \
-                    ns.photometric and ns.overlap and hasattr(optimizer, "advance")
+                    ns.photometric and ns.overlap and hasattr(optimizer, "advance") and optimizer.max_grad_norm is None
+                # (clipping needs every gradient before the first parameter is updated: the update is then one call behind the backward)
                 ns.step_optimizer = optimizer if split else None
                 # the carried texture (step.py: enable_carry): the finish + Adam pass hands the next replay its albedo + pyramid level 1;
                 # replays prime it when they cannot know it is current (_carry_prime_if_needed)
@@ -1417,7 +1428,7 @@ class GraphedStep:
                 T = int(tracker.tex_extra.shape[-1]) if tracker.tex_extra is not None else 0
                 tex = tracker.tex_extra
                 self.tex_sharded = bool(ns.tex_bwd_on and ns.pca is None and tex is not None and any(p is tex for p in self.params) and T % (16 * world) == 0 and
-                                        isinstance(optimizer, NV.HipAdam) and os.environ.get("VHAP_TEX_SHARDED", "1") != "0")
+                                        isinstance(optimizer, NV.HipAdam) and optimizer.max_grad_norm is None and os.environ.get("VHAP_TEX_SHARDED", "1") != "0")
                 if self.tex_sharded and not tracker.dist.tex_sharded_usable():   # (every collective of the path once, on small tensors, all ranks together)
                     self.tex_sharded = False
                 if self.tex_sharded:
@@ -1540,6 +1551,7 @@ class GraphedStep:
                         p.grad = torch.zeros_like(p)
                 self.E = E.detach()
             with self.gA.capture(pool=pool, **cap):
+                tracker.clip_gradients(optimizer)
                 optimizer.step()
         finally:
             tracker._split = None
