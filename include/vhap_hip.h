@@ -712,14 +712,14 @@ int vhap_adam_step(int n_tensors, float* const* params, const float* const* grad
  *   norm = (sum |g|^p)^(1/p) over ALL elements of all tensors (norm_kind 1 or 2), or max |g| (VHAP_NORM_INF); summed in 64 bits, in a fixed order
  *   c = min(1, max_norm / (norm + 1e-6)); a NaN norm makes c NaN; an infinite one makes it 0 (and 0 x infinity NaN)
  * grads[k]: numel[k] consecutive elements of dtype[k] (VHAP_DTYPE_*; dtype NULL: all float32), aligned to their element; any number of tensors, empty ones
- * among them; fewer than 2^39 elements in all.  norm: device float, overwritten.  workspace: vhap_grad_norm_workspace_bytes(n_tensors), not shared by
+ * among them; fewer than 2^38 elements in all.  norm: device float, overwritten.  workspace: vhap_grad_norm_workspace_bytes(n_tensors), not shared by
  * calls in flight at the same time.
  * vhap_grad_clip: out[k] = round(grads[k] * c) to the same dtype; out[k] is grads[k] itself (in place; a list that is not clipped is then not rewritten) or
  *   memory of its own: VHAP_E_UNSUPPORTED where a destination overlaps another destination or another tensor's source.  max_norm >= 0.
  * vhap_adam_step_clipped: vhap_adam_step on round(grads * c), the gradients left as they are, the norm over these n_tensors (2-norm; norm may be NULL):
  *   the counter is advanced by the call's own launches (no third one).  call_flags as vhap_adam_step.  The hyperparameters are 64-bit: 1 - beta and
  *   1 - beta^step are formed there and rounded to float32 once (vhap_adam_step forms them in float32: its 1 - beta2 is off by 1.3e-5 at beta2 = 0.999).
- * Lists of at most 32768 elements (by units of 512 a tensor) are one launch, others two, and two more for every further 128 tensors that do not lie one
+ * Lists of at most 64 units of 2 KB (no unit crosses a tensor) are one launch, others two, and two more for every further 128 tensors that do not lie one
  * behind another in memory. */
 #define VHAP_NORM_INF 0
 #define VHAP_DTYPE_F32 0

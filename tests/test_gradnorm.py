@@ -49,7 +49,9 @@ LISTS = {
     "empty_among": [((0,), torch.float32), ((5,), torch.float32), ((3, 0), torch.bfloat16), ((1000,), torch.float32)],
     "tracker": [((300,), torch.float32), ((16, 100), torch.float32), ((16, 3), torch.float32), ((1,), torch.float32), ((1, 5143, 3), torch.float32), ((3, 257, 255), torch.float32)],
     "one_block_border": [((32768,), torch.float32)],
-    "past_one_block": [((32769,), torch.bfloat16)],
+    "past_one_block": [((32769,), torch.float32)],
+    "one_block_border_16": [((65536,), torch.bfloat16)],
+    "past_one_block_16": [((65535,), torch.float16), ((1,), torch.bfloat16)],
     "large_mixed": [((1 << 20,), torch.float32), ((123457,), torch.float16), ((3, 1025, 333), torch.bfloat16)],
 }
 
@@ -100,8 +102,8 @@ def test_c_entry_refusals():
     big = 1 << 20                                                    # (more than one block's work: a workspace is needed)
     assert _c_clip([B], [B], [big]) == _lib.E_WORKSPACE
     assert _c_clip([B], [B], [-1]) == _lib.E_BADDIM
-    assert _c_clip([B], [B], [1 << 39]) == _lib.E_BADDIM
-    assert _c_clip([B, B], [B, B], [1 << 38, 1 << 38]) == _lib.E_BADDIM
+    assert _c_clip([B], [B], [1 << 38]) == _lib.E_BADDIM
+    assert _c_clip([B, B], [B, B], [1 << 37, 1 << 37]) == _lib.E_BADDIM
     assert _c_clip([B], [B], [big], dtype=[3]) == _lib.E_BADDIM
     assert _c_clip([B], [B], [big], max_norm=-1.0) == _lib.E_BADDIM
     assert _c_clip([B], [B], [big], max_norm=math.nan) == _lib.E_BADDIM
@@ -148,6 +150,20 @@ def test_norm_and_clip(name, p, share):
     assert torch.equal(n, n2)
     for o, g in zip(out, gs):
         assert torch.equal(o, g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("share", [0.5, 2.0])
+def test_some_in_place_some_not(share):
+    """one list, a large tensor in place beside one that is not, clipped and within the limit (where the first is left alone and the second copied)"""
+    gs = [randn((1 << 21,), 1), randn((1 << 21,), 2), randn((3, 1000, 1001), 3, torch.bfloat16)]
+    keep = [g.clone() for g in gs]
+    want = norm64(keep, 2.0)
+    out = [gs[0], torch.zeros_like(gs[1]), gs[2]]
+    n = NV.clip_by_global_norm(gs, want * share, out=out)[1]
+    assert near_norm(float(n), want) and torch.equal(gs[1], keep[1])
+    for o, k in zip(out, keep):
+        check_clipped(o, k, coefficient(want, want * share))
 
 
 @pytest.mark.gpu

@@ -222,7 +222,7 @@ def host():
         loader = importlib.machinery.ExtensionFileLoader("vhap_host", path)
         m = importlib.util.module_from_spec(importlib.util.spec_from_loader("vhap_host", loader))
         loader.exec_module(m)
-        names = [n for n in SIGNATURES if n == "vhap_strerror" or n.startswith(("vhap_grad_", "vhap_mx4_"))]
+        names = [n for n in SIGNATURES if n == "vhap_strerror" or n.startswith(("vhap_grad_", "vhap_mx4_", "vhap_adam_step_clipped"))]
         m.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names}, VhapHipError)
         _host = m
     return _host

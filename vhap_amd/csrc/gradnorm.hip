@@ -4,25 +4,25 @@
 //   c = min(1, max_norm / (n + 1e-6)), NaN where n is NaN;   out = round(g c)   or   Adam on round32(g c)
 //
 // HBM-bound: the list is read once for n and once for out (the second time from the cache in front of HBM up to some 100 MB), written once.
-// The list is cut into units of 512 elements that never cross a tensor; a WAVE owns a contiguous run of units, so one launch serves tensors of
-// any sizes side by side (one block per tensor or per 4096 elements would leave most lanes of a tracker's ten small tensors idle).  512 blocks
-// of 16 waves fill the chip and leave 512 partial sums: every block of the second launch adds those up itself, in the same order (4 KB out of L2), so
-// there is no third launch, no counter and no atomic -- the same call gives the same bits.
+// The list is cut into units of 2 KB that never cross a tensor; a WAVE owns a contiguous run of units, so one launch serves tensors of any sizes and types side
+// by side (a block per tensor would leave most lanes of a tracker's ten small tensors idle).  A unit is two 16-byte loads a lane, four whole units of one tensor
+// are read at a time.  256 blocks of 16 waves fill the chip and leave 256 partial sums: every block of the second launch adds those up itself, in the same order
+// (2 KB out of L2), with its first four units already on their way, so there is no third launch, no counter and no atomic -- the same call gives the same bits.
 // The sums are held in 64 bits: the square of an fp32 number is exact there, and no finite gradient overflows.  n is rounded to fp32 once; c is formed
 // from the 64-bit n and rounded to fp32 once.
 // Lists of at most ONE_BLOCK_UNITS units are one block's work in ONE launch (norm, barrier, scale): what counts there is the launches.
-// Measurements: see the bottom of this comment's table in the entry points.
 #include "common.h"
 #include "elem8.h"
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 namespace {
 
-constexpr int GN_T = 1024, GN_WAVES = GN_T / 64, GN_BLOCKS = 512, GN_UNIT = 512;
+constexpr int GN_T = 1024, GN_WAVES = GN_T / 64, GN_BLOCKS = 256, GN_UNIT = 2048;
 constexpr int GN_MAX = 128;                 // tensors per launch: the table travels as kernel arguments (under 4 KB), so a capture keeps it by value
-constexpr long long GN_MOST = 1ll << 39;    // elements of a list: its units are counted in 32 bits
+constexpr long long GN_MOST = 1ll << 38;    // elements of a list: its units are counted in 32 bits
 constexpr int ONE_BLOCK_UNITS = 64;
 
 template <int MAX>
@@ -30,12 +30,14 @@ struct GnTableOf {
     const void* src[MAX];
     void* dst[MAX];                         // norm only: unused
     long long n[MAX];
-    unsigned start[MAX + 1];                // first unit of tensor k
+    unsigned start[MAX + 1];                // first unit (of GN_UNIT bytes) of tensor k
     unsigned char dtype[MAX];
     int count;
 };
 using GnTable = GnTableOf<GN_MAX>;
 using GnAdamTable = GnTableOf<VHAP_ADAM_MAX_TENSORS>;
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // KIND: 0 = infinity, 1, 2.  An accumulator is a double; for the maximum it holds the BITS of |g| as an integer value: bits order like the numbers they
 // stand for and a NaN lies above infinity, so that it wins the maximum.
@@ -46,6 +48,81 @@ __device__ __forceinline__ double gn_take(double a, float x) {
     if constexpr (KIND == 0) return gn_join<0>(a, (double)(__float_as_uint(x) & 0x7fffffffu));
     if constexpr (KIND == 1) return a + (double)fabsf(x);
     return fma((double)x, (double)x, a);
+}
+
+// 16 bytes as four fp32 or eight bf16 / fp16 numbers
+template <int DT>
+constexpr int gn_count() { return DT == VHAP_DTYPE_F32 ? 4 : 8; }
+template <int DT>
+__device__ __forceinline__ void gn_floats(const u32x4& r, float (&v)[gn_count<DT>()]) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (DT == VHAP_DTYPE_F32) v[k] = __uint_as_float(r[k]);
+        if constexpr (DT == VHAP_DTYPE_BF16) { v[2 * k] = __uint_as_float(r[k] << 16); v[2 * k + 1] = __uint_as_float(r[k] & 0xffff0000u); }
+        if constexpr (DT == VHAP_DTYPE_F16) {
+            v[2 * k] = __half2float(__ushort_as_half((unsigned short)(r[k] & 0xffffu)));
+            v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(r[k] >> 16)));
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ u32x4 gn_bits(const float (&v)[gn_count<DT>()]) {
+    u32x4 r;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (DT == VHAP_DTYPE_F32) r[k] = __float_as_uint(v[k]);
+        if constexpr (DT == VHAP_DTYPE_BF16) r[k] = vhap_bf16_pair(v[2 * k], v[2 * k + 1]);
+        if constexpr (DT == VHAP_DTYPE_F16) r[k] = (unsigned)__half_as_ushort(__float2half_rn(v[2 * k])) | (unsigned)__half_as_ushort(__float2half_rn(v[2 * k + 1])) << 16;
+    }
+    return r;
+}
+template <int KIND, int DT>
+__device__ __forceinline__ void gn_take16(double (&a)[2], const u32x4& r) {
+    float v[gn_count<DT>()];
+    gn_floats<DT>(r, v);
+#pragma unroll
+    for (int e = 0; e < gn_count<DT>(); e++) a[e & 1] = gn_take<KIND>(a[e & 1], v[e]);
+}
+template <int DT>
+__device__ __forceinline__ u32x4 gn_scale16(const u32x4& r, float c) {
+    float v[gn_count<DT>()];
+    gn_floats<DT>(r, v);
+#pragma unroll
+    for (int e = 0; e < gn_count<DT>(); e++) v[e] *= c;
+    return gn_bits<DT>(v);
+}
+
+typedef u32x4 __attribute__((aligned(2))) gn_any;        // at any address its elements may have: 16-byte accesses need no more on this target
+__device__ __forceinline__ u32x4 gn_load(const char* p) { return *reinterpret_cast<const gn_any*>(p); }
+__device__ __forceinline__ void gn_store(char* p, const u32x4& v) { *reinterpret_cast<gn_any*>(p) = v; }
+// the last, partial unit of a tensor: `bytes` of the 16 at p exist
+template <int DT>
+__device__ __forceinline__ u32x4 gn_load_part(const char* p, int bytes) {
+    u32x4 r = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (DT == VHAP_DTYPE_F32) {
+            if (4 * k < bytes) r[k] = reinterpret_cast<const unsigned*>(p)[k];
+        } else {
+            const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+            if (4 * k < bytes) r[k] = h[2 * k];
+            if (4 * k + 2 < bytes) r[k] |= (unsigned)h[2 * k + 1] << 16;
+        }
+    }
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void gn_store_part(char* p, int bytes, const u32x4& r) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (DT == VHAP_DTYPE_F32) {
+            if (4 * k < bytes) reinterpret_cast<unsigned*>(p)[k] = r[k];
+        } else {
+            unsigned short* h = reinterpret_cast<unsigned short*>(p);
+            if (4 * k < bytes) h[2 * k] = (unsigned short)(r[k] & 0xffffu);
+            if (4 * k + 2 < bytes) h[2 * k + 1] = (unsigned short)(r[k] >> 16);
+        }
+    }
 }
 
 // sum (or maximum) over the block, in every thread; the waves are joined in order
@@ -71,32 +148,62 @@ __device__ __forceinline__ int gn_find(const Table& t, unsigned unit) {       //
     return lo;
 }
 
-// this wave's run of units, f(tensor, first element of this lane's eight, how many of them exist)
+// This wave's run of units, piece by piece: f(tensor, byte offset of the piece, whole units in it (1 .. 4), bytes of a partial one (whole units: 0)).  All of it is the
+// same for the wave.
 template <typename Table, typename F>
-__device__ __forceinline__ void gn_units(const Table& t, unsigned wave, unsigned nwaves, F f) {
+__device__ __forceinline__ void gn_pieces(const Table& t, unsigned wave, unsigned nwaves, F f) {
     const unsigned units = t.start[t.count];
     unsigned u = (unsigned)((unsigned long long)units * wave / nwaves);
     const unsigned u1 = (unsigned)((unsigned long long)units * (wave + 1) / nwaves);
     if (u >= u1) return;
     int k = gn_find(t, u);
-    for (; u < u1; u++) {
+    while (u < u1) {
         while (u >= t.start[k + 1]) k++;
-        const long long i = (long long)(u - t.start[k]) * GN_UNIT + (threadIdx.x & 63) * 8;
-        const long long left = t.n[k] - i;
-        if (left > 0) f(k, i, left < 8 ? (int)left : 8);
+        const long long bytes = t.n[k] * (t.dtype[k] == VHAP_DTYPE_F32 ? 4 : 2), at = (long long)(u - t.start[k]) * GN_UNIT;
+        const unsigned whole = (unsigned)min((bytes - at) / GN_UNIT, (long long)(u1 - u));
+        if (whole == 0) {
+            f(k, at, 0, (int)(bytes - at));
+            u++;
+        } else {
+            const int n = whole >= 4 ? 4 : 1;
+            f(k, at, n, 0);
+            u += n;
+        }
     }
+}
+// f<type>() by a tensor's type
+template <typename F>
+__device__ __forceinline__ void gn_by_type(int dt, F f) {
+    if (dt == VHAP_DTYPE_F32) f(std::integral_constant<int, VHAP_DTYPE_F32>());
+    else if (dt == VHAP_DTYPE_BF16) f(std::integral_constant<int, VHAP_DTYPE_BF16>());
+    else f(std::integral_constant<int, VHAP_DTYPE_F16>());
 }
 
 template <int KIND, typename Table>
 __device__ __forceinline__ double gn_wave_part(const Table& t, unsigned wave, unsigned nwaves) {
-    double a0 = 0., a1 = 0.;
-    gn_units(t, wave, nwaves, [&](int k, long long i, int valid) {
-        float v[8];
-        vhap_load8(t.src[k], i, t.dtype[k], valid, v);
+    double a[2] = {0., 0.};
+    const int lane = (threadIdx.x & 63) * 16;
+    gn_pieces(t, wave, nwaves, [&](int k, long long at, int whole, int part) {
+        const char* p = static_cast<const char*>(t.src[k]) + at + lane;
+        gn_by_type(t.dtype[k], [&](auto type) {
+            constexpr int DT = decltype(type)::value;
+            if (whole == 4) {
+                u32x4 r[8];
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) { a0 = gn_take<KIND>(a0, v[e]); a1 = gn_take<KIND>(a1, v[e + 1]); }
+                for (int h = 0; h < 8; h++) r[h] = gn_load(p + h * 1024);
+#pragma unroll
+                for (int h = 0; h < 8; h++) gn_take16<KIND, DT>(a, r[h]);
+            } else if (whole) {
+                const u32x4 r0 = gn_load(p), r1 = gn_load(p + 1024);
+                gn_take16<KIND, DT>(a, r0);
+                gn_take16<KIND, DT>(a, r1);
+            } else {
+                gn_take16<KIND, DT>(a, gn_load_part<DT>(p, part - lane));
+                gn_take16<KIND, DT>(a, gn_load_part<DT>(p + 1024, part - lane - 1024));
+            }
+        });
     });
-    return gn_join<KIND>(a0, a1);
+    return gn_join<KIND>(a[0], a[1]);
 }
 
 template <int KIND>
@@ -142,16 +249,52 @@ template <int KIND>
 __global__ __launch_bounds__(GN_T) void gn_scale_kernel(const GnTable t, const double* __restrict__ part, int n_part, double max_norm, float* __restrict__ norm) {
     __shared__ double lds[GN_WAVES];
     const unsigned wave = __builtin_amdgcn_readfirstlane(blockIdx.x * GN_WAVES + (threadIdx.x >> 6));
+    const int lane = (threadIdx.x & 63) * 16;
+    // the first piece, if it is four whole units, is on its way while the norm is put together
+    u32x4 ahead[8];
+    bool have = false;
+    if (part) {
+        const unsigned units = t.start[t.count], waves = gridDim.x * GN_WAVES;
+        const unsigned u = (unsigned)((unsigned long long)units * wave / waves), u1 = (unsigned)((unsigned long long)units * (wave + 1) / waves);
+        if (u + 4 <= u1) {
+            const int k = gn_find(t, u);
+            const long long bytes = t.n[k] * (t.dtype[k] == VHAP_DTYPE_F32 ? 4 : 2), at = (long long)(u - t.start[k]) * GN_UNIT;
+            have = bytes - at >= 4 * GN_UNIT;
+            if (have) {
+                const char* p = static_cast<const char*>(t.src[k]) + at + lane;
+#pragma unroll
+                for (int h = 0; h < 8; h++) ahead[h] = gn_load(p + h * 1024);
+            }
+        }
+    }
     const double n = part ? gn_total<KIND>(part, n_part, lds) : gn_norm_of<KIND>(gn_block_join<KIND>(gn_wave_part<KIND>(t, wave, GN_WAVES), lds));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)n;
     const float c = gn_coefficient(n, max_norm);
-    gn_units(t, wave, gridDim.x * GN_WAVES, [&](int k, long long i, int valid) {
+    gn_pieces(t, wave, gridDim.x * GN_WAVES, [&](int k, long long at, int whole, int part_bytes) {
+        const bool loaded = have;
+        have = false;                                                     // (the first piece's alone, whether it is used or not)
         if (c == 1.0f && t.src[k] == t.dst[k]) return;                    // in place and not clipped: every element keeps its value
-        float v[8];
-        vhap_load8(t.src[k], i, t.dtype[k], valid, v);
+        const char* p = static_cast<const char*>(t.src[k]) + at + lane;
+        char* o = static_cast<char*>(t.dst[k]) + at + lane;
+        gn_by_type(t.dtype[k], [&](auto type) {
+            constexpr int DT = decltype(type)::value;
+            if (whole == 4) {
+                if (!loaded) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] *= c;
-        vhap_store8(t.dst[k], i, t.dtype[k], valid, v);
+                    for (int h = 0; h < 8; h++) ahead[h] = gn_load(p + h * 1024);
+                }
+#pragma unroll
+                for (int h = 0; h < 8; h++) gn_store(o + h * 1024, gn_scale16<DT>(ahead[h], c));
+            } else if (whole) {
+                const u32x4 r0 = gn_load(p), r1 = gn_load(p + 1024);
+                gn_store(o, gn_scale16<DT>(r0, c));
+                gn_store(o + 1024, gn_scale16<DT>(r1, c));
+            } else {
+                const u32x4 r0 = gn_load_part<DT>(p, part_bytes - lane), r1 = gn_load_part<DT>(p + 1024, part_bytes - lane - 1024);
+                gn_store_part<DT>(o, part_bytes - lane, gn_scale16<DT>(r0, c));
+                gn_store_part<DT>(o + 1024, part_bytes - lane - 1024, gn_scale16<DT>(r1, c));
+            }
+        });
     });
 }
 
@@ -183,28 +326,46 @@ __global__ __launch_bounds__(GN_T) void gn_adam_kernel(const GnAdamTable t, cons
     if (bump && threadIdx.x == 0) step[0] += 1;          // (one block; what reads the counter has done so: the join above is a barrier)
     const float c = gn_coefficient(n, max_norm);
     const float bc1 = bias_correction[0], bc2s = bias_correction[1], b2 = (float)beta2, left1 = (float)(1.0 - beta1), left2 = (float)(1.0 - beta2);
-    gn_units(t, wave, gridDim.x * GN_WAVES, [&](int k, long long i, int valid) {
+    const int lane = (threadIdx.x & 63) * 16;
+    gn_pieces(t, wave, gridDim.x * GN_WAVES, [&](int k, long long at0, int whole, int part_bytes) {
         const float step_size = lr[a.lr_index[k]] / bc1;
-        float g[8], p[8], m[8], v[8];
-        vhap_load8(t.src[k], i, VHAP_DTYPE_F32, valid, g);
-        vhap_load8(a.p[k], i, VHAP_DTYPE_F32, valid, p);
-        vhap_load8(a.m[k], i, VHAP_DTYPE_F32, valid, m);
-        vhap_load8(a.v[k], i, VHAP_DTYPE_F32, valid, v);
+        for (int w = 0; w < (whole ? whole : 1); w++) {
+            const long long at = at0 + (long long)w * GN_UNIT + lane;
+            const char* src[4] = {static_cast<const char*>(t.src[k]) + at, reinterpret_cast<char*>(a.p[k]) + at, reinterpret_cast<char*>(a.m[k]) + at,
+                                  reinterpret_cast<char*>(a.v[k]) + at};
+            u32x4 r[4][2];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float gi = gn_mul(g[e], c);         // the clipped gradient as clipping in place would have stored it
-            m[e] = m[e] + (gi - m[e]) * left1;
-            v[e] = b2 * v[e] + left2 * gi * gi;
-            p[e] -= step_size * m[e] / (sqrtf(v[e]) / bc2s + eps);
+            for (int x = 0; x < 4; x++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    r[x][h] = whole ? gn_load(src[x] + h * 1024) : gn_load_part<VHAP_DTYPE_F32>(src[x] + h * 1024, part_bytes - lane - h * 1024);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float g[4], p[4], m[4], v[4];
+                gn_floats<VHAP_DTYPE_F32>(r[0][h], g);
+                gn_floats<VHAP_DTYPE_F32>(r[1][h], p);
+                gn_floats<VHAP_DTYPE_F32>(r[2][h], m);
+                gn_floats<VHAP_DTYPE_F32>(r[3][h], v);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float gi = gn_mul(g[e], c);    // the clipped gradient as clipping in place would have stored it
+                    m[e] = m[e] + (gi - m[e]) * left1;
+                    v[e] = b2 * v[e] + left2 * gi * gi;
+                    p[e] -= step_size * m[e] / (sqrtf(v[e]) / bc2s + eps);
+                }
+                const u32x4 out[3] = {gn_bits<VHAP_DTYPE_F32>(p), gn_bits<VHAP_DTYPE_F32>(m), gn_bits<VHAP_DTYPE_F32>(v)};
+#pragma unroll
+                for (int x = 0; x < 3; x++) {
+                    if (whole) gn_store(const_cast<char*>(src[x + 1]) + h * 1024, out[x]);
+                    else gn_store_part<VHAP_DTYPE_F32>(const_cast<char*>(src[x + 1]) + h * 1024, part_bytes - lane - h * 1024, out[x]);
+                }
+            }
         }
-        vhap_store8(a.m[k], i, VHAP_DTYPE_F32, valid, m);
-        vhap_store8(a.v[k], i, VHAP_DTYPE_F32, valid, v);
-        vhap_store8(a.p[k], i, VHAP_DTYPE_F32, valid, p);
     });
 }
 
 // ---- host side ----
-inline long long gn_units_of(long long n) { return (n + GN_UNIT - 1) / GN_UNIT; }
+inline long long gn_units_of(long long n, int size) { return (n * size + GN_UNIT - 1) / GN_UNIT; }
 
 // Walks the list in launches of at most MAX entries, f(table, units); entries that lie one behind another in memory (views of one flat buffer, source
 // and destination alike) are one entry.
@@ -221,7 +382,7 @@ int gn_walk(int n_tensors, const void* const* src, void* const* dst, const int64
             const long long was = t.n[j] * size;
             if (t.dtype[j] == dt && static_cast<const char*>(t.src[j]) + was == src[k] && (!dst || static_cast<char*>(t.dst[j]) + was == dst[k])) {
                 t.n[j] += numel[k];
-                units = t.start[j] + (unsigned)gn_units_of(t.n[j]);
+                units = t.start[j] + (unsigned)gn_units_of(t.n[j], size);
                 continue;
             }
         }
@@ -238,7 +399,7 @@ int gn_walk(int n_tensors, const void* const* src, void* const* dst, const int64
         t.n[j] = numel[k];
         t.dtype[j] = (unsigned char)dt;
         t.start[j] = units;
-        units += (unsigned)gn_units_of(numel[k]);
+        units += (unsigned)gn_units_of(numel[k], size);
     }
     if (t.count == 0) return VHAP_OK;
     t.start[t.count] = units;

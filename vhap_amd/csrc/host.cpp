@@ -26,6 +26,7 @@ struct Api {
     decltype(&vhap_grad_norm_workspace_bytes) norm_bytes = nullptr;
     decltype(&vhap_grad_norm) norm = nullptr;
     decltype(&vhap_grad_clip) clip = nullptr;
+    decltype(&vhap_adam_step_clipped) adam = nullptr;
     decltype(&vhap_mx4_quantize) quantize = nullptr;
     decltype(&vhap_mx4_dequantize) dequantize = nullptr;
     decltype(&vhap_mx4_linear) linear = nullptr;
@@ -62,25 +63,31 @@ void on_hip(const Tensor& t, const char* what) {
 }
 
 // ---- the global norm ----
-using List = std::vector<Tensor>;
+// The tensors of a Python sequence, borrowed: `keep` holds the sequence, which holds them.
+struct List {
+    py::object keep;
+    std::vector<const Tensor*> t;
+    size_t size() const { return t.size(); }
+    const Tensor& operator[](size_t i) const { return *t[i]; }
+};
 
 List gradients(py::handle given, const char* what) {
-    List ts;
-    py::object seq = py::reinterpret_steal<py::object>(PySequence_Fast(given.ptr(), "expected a sequence of tensors"));
-    if (!seq) throw py::error_already_set();
-    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq.ptr());
-    ts.reserve(n);
+    List l;
+    l.keep = py::reinterpret_steal<py::object>(PySequence_Fast(given.ptr(), "expected a sequence of tensors"));
+    if (!l.keep) throw py::error_already_set();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(l.keep.ptr());
+    PyObject** items = PySequence_Fast_ITEMS(l.keep.ptr());
+    l.t.reserve(n);
     for (Py_ssize_t i = 0; i < n; i++) {
-        PyObject* o = PySequence_Fast_GET_ITEM(seq.ptr(), i);
-        if (!THPVariable_Check(o)) throw py::type_error(text(what, ": expected tensors, got ", Py_TYPE(o)->tp_name));
-        const Tensor& t = THPVariable_Unpack(o);
+        if (!THPVariable_Check(items[i])) throw py::type_error(text(what, ": expected tensors, got ", Py_TYPE(items[i])->tp_name));
+        const Tensor& t = THPVariable_Unpack(items[i]);
         if (t.layout() != at::kStrided || dtype_code(t.scalar_type()) < 0)
             throw py::type_error(text(what, ": dense float32, bfloat16 or float16 tensors, got ", t.scalar_type(), " (", t.layout(), ")"));
         on_hip(t, what);
-        if (i > 0 && t.device() != ts[0].device()) throw py::value_error(text(what, ": tensors on one device, got ", ts[0].device(), " and ", t.device()));
-        ts.push_back(t);
+        if (i > 0 && t.device() != l[0].device()) throw py::value_error(text(what, ": tensors on one device, got ", l[0].device(), " and ", t.device()));
+        l.t.push_back(&t);
     }
-    return ts;
+    return l;
 }
 
 struct Table {
@@ -88,6 +95,12 @@ struct Table {
     std::vector<void*> dst;
     std::vector<int64_t> numel;
     std::vector<int32_t> dtype;
+    explicit Table(size_t n) {
+        src.reserve(n);
+        dst.reserve(n);
+        numel.reserve(n);
+        dtype.reserve(n);
+    }
     void add(const Tensor& s, const Tensor* d) {
         src.push_back(s.data_ptr());
         if (d) dst.push_back(d->data_ptr());
@@ -100,13 +113,18 @@ Tensor workspace(size_t bytes, const Tensor& like) { return at::empty({(int64_t)
 
 Tensor grad_norm(py::handle given, int kind) {
     at::NoGradGuard no_grad;
-    List ts = gradients(given, "grad_norm");
-    if (ts.empty()) return at::zeros({});
+    const List ts = gradients(given, "grad_norm");
+    if (ts.size() == 0) return at::zeros({});
     c10::DeviceGuard guard(ts[0].device());
-    Table t;
-    for (Tensor& x : ts) {
-        if (!x.is_non_overlapping_and_dense()) x = x.contiguous();
-        t.add(x, nullptr);
+    Table t(ts.size());
+    std::vector<Tensor> copies;
+    for (size_t i = 0; i < ts.size(); i++) {
+        if (ts[i].is_non_overlapping_and_dense()) {
+            t.add(ts[i], nullptr);
+        } else {
+            copies.push_back(ts[i].contiguous());
+            t.add(copies.back(), nullptr);
+        }
     }
     const size_t bytes = api.norm_bytes((int)ts.size());
     Tensor ws = workspace(bytes, ts[0]), norm = at::empty({}, ts[0].options().dtype(at::kFloat));
@@ -118,13 +136,18 @@ Tensor grad_norm(py::handle given, int kind) {
 py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
     at::NoGradGuard no_grad;
     static const char* what = "clip_by_global_norm";
-    List gs = gradients(given, what), outs;
+    const List gs = gradients(given, what);
     const bool made = out.is_none(), in_place = !made && out.ptr() == given.ptr();
+    std::vector<Tensor> fresh;
+    List outs;
     if (made) {
-        outs.reserve(gs.size());
-        for (const Tensor& g : gs) outs.push_back(at::empty(g.sizes(), g.options()));
+        fresh.reserve(gs.size());
+        for (size_t i = 0; i < gs.size(); i++) {
+            fresh.push_back(at::empty(gs[i].sizes(), gs[i].options()));
+            outs.t.push_back(&fresh.back());
+        }
     } else if (in_place) {
-        outs = gs;
+        outs.t = gs.t;
     } else {
         outs = gradients(out, "clip_by_global_norm(out=)");
         if (outs.size() != gs.size()) throw py::value_error(text(what, ": ", gs.size(), " gradients, ", outs.size(), " results"));
@@ -133,14 +156,14 @@ py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
                 throw py::value_error(text(what, ": a result is like its gradient: ", gs[i].sizes(), " ", gs[i].scalar_type(), " ", gs[i].device(), ", got ", outs[i].sizes(), " ",
                                            outs[i].scalar_type(), " ", outs[i].device()));
     }
-    py::object results = made ? py::cast(outs) : in_place ? py::reinterpret_borrow<py::object>(given) : out;
-    if (gs.empty()) return py::make_tuple(results, at::zeros({}));
+    py::object results = made ? py::cast(fresh) : in_place ? py::reinterpret_borrow<py::object>(given) : out;
+    if (gs.size() == 0) return py::make_tuple(results, at::zeros({}));
     c10::DeviceGuard guard(gs[0].device());
     // the kernels walk memory in order: a pair that is dense with the same strides is taken as it stands, anything else goes through contiguous copies
-    Table t;
+    Table t(gs.size());
     std::vector<std::pair<Tensor, Tensor>> back;
     std::set<std::tuple<const void*, std::vector<int64_t>, std::vector<int64_t>>> strided;
-    List keep;
+    std::vector<Tensor> keep;
     for (size_t i = 0; i < gs.size(); i++) {
         const Tensor &g = gs[i], &o = outs[i];
         if ((g.is_contiguous() && o.is_contiguous()) || (g.strides() == o.strides() && g.is_non_overlapping_and_dense())) {
@@ -156,17 +179,43 @@ py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
         back.emplace_back(o, r);
     }
     const size_t bytes = api.norm_bytes((int)gs.size());
-    Tensor ws = workspace(bytes, gs[0]), norm = at::empty({}, gs[0].options().dtype(at::kFloat));
+    const Tensor ws = workspace(bytes, gs[0]), norm = at::empty({}, gs[0].options().dtype(at::kFloat));
     const int rc = api.clip((int)gs.size(), t.src.data(), t.dst.data(), t.numel.data(), t.dtype.data(), kind, max_norm, ws.data_ptr(), bytes, norm.data_ptr<float>(),
                             stream_of(norm));
     if (rc == VHAP_E_UNSUPPORTED) throw py::value_error("clipping: a result overlaps another result, or another gradient, in memory (the same tensor twice in the list?)");
     check(rc, "vhap_grad_clip");
     for (auto& b : back) b.first.copy_(b.second);
     if (!made)
-        for (const Tensor& o : outs)
-            if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();       // (written behind autograd's back)
+        for (const Tensor* o : outs.t)
+            if (!o->is_inference()) o->unsafeGetTensorImpl()->bump_version();       // (written behind autograd's back)
     return py::make_tuple(results, norm);
 }
+
+// What vhap_adam_step_clipped reads of an optimiser, per set of parameters that have a gradient; the gradients come with every step.
+struct AdamTable {
+    std::vector<float*> p, m, v;
+    std::vector<int64_t> numel;
+    std::vector<int32_t> lr_index;
+    AdamTable(const std::vector<uintptr_t>& ps, const std::vector<uintptr_t>& ms, const std::vector<uintptr_t>& vs, std::vector<int64_t> n, std::vector<int32_t> lr)
+        : numel(std::move(n)), lr_index(std::move(lr)) {
+        for (uintptr_t x : ps) p.push_back(reinterpret_cast<float*>(x));
+        for (uintptr_t x : ms) m.push_back(reinterpret_cast<float*>(x));
+        for (uintptr_t x : vs) v.push_back(reinterpret_cast<float*>(x));
+    }
+    void step(py::handle grads, const Tensor& lr, const Tensor& step, double beta1, double beta2, double eps, double max_norm, const Tensor& ws, const Tensor& norm, int flags) const {
+        const List g = gradients(grads, "HipAdam");
+        if (g.size() != p.size()) throw py::value_error("HipAdam: a gradient for every parameter of the table");
+        std::vector<const float*> gp(g.size());
+        for (size_t i = 0; i < g.size(); i++) {
+            if (g[i].scalar_type() != at::kFloat || !g[i].is_contiguous() || g[i].numel() != numel[i] || g[i].device() != norm.device())
+                throw std::runtime_error("HipAdam needs contiguous float32 gradients like its parameters");
+            gp[i] = static_cast<const float*>(g[i].data_ptr());
+        }
+        c10::DeviceGuard guard(norm.device());
+        check(api.adam((int)g.size(), p.data(), gp.data(), m.data(), v.data(), numel.data(), lr_index.data(), lr.data_ptr<float>(), step.data_ptr<int32_t>(), beta1, beta2, eps,
+                       max_norm, ws.data_ptr(), (size_t)ws.nbytes(), norm.data_ptr<float>(), flags, stream_of(norm)), "vhap_adam_step_clipped");
+    }
+};
 
 // ---- 4-bit products ----
 // [..., K] -> (rows, row stride): a matrix with consecutive elements along K; anything else is copied
@@ -315,6 +364,7 @@ void bind(const py::dict& at, py::object error) {
     take(api.norm_bytes, "vhap_grad_norm_workspace_bytes");
     take(api.norm, "vhap_grad_norm");
     take(api.clip, "vhap_grad_clip");
+    take(api.adam, "vhap_adam_step_clipped");
     take(api.quantize, "vhap_mx4_quantize");
     take(api.dequantize, "vhap_mx4_dequantize");
     take(api.linear, "vhap_mx4_linear");
@@ -338,6 +388,9 @@ PYBIND11_MODULE(vhap_host, m) {
     m.def("bind", &bind);
     m.def("grad_norm", &grad_norm);
     m.def("clip", &clip);
+    py::class_<AdamTable>(m, "AdamTable")
+        .def(py::init<std::vector<uintptr_t>, std::vector<uintptr_t>, std::vector<uintptr_t>, std::vector<int64_t>, std::vector<int32_t>>())
+        .def("step", &AdamTable::step);
     m.def("quantize", &quantize);
     m.def("dequantize", &dequantize);
     m.def("linear", &linear);

@@ -12,7 +12,6 @@ Together they replace the several hundred tiny eager launches per step that the 
     grad_norm, clip_by_global_norm, clip_grad_norm_
                      the norm over a list of gradients and the list scaled to a largest one (vhap_amd/csrc/gradnorm.hip)
 """
-import contextlib
 import ctypes
 import math
 import os
@@ -379,13 +378,7 @@ def tex_prep(painted, extra, res_mask_u8, w_tv, w_res, scales=None):
 
 # ------------------------------------------------------------------------------------------------
 # ---- the global norm over many gradients, and clipping ----
-_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # VHAP_DTYPE_*
 _NORM_KIND = {1.0: 1, 2.0: 2, math.inf: 0}                                   # VHAP_NORM_INF = 0
-
-
-def on_device(t):
-    """context in which the current device (and so the current stream) is that of tensor `t`"""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _tensors(ts):
@@ -586,19 +579,18 @@ class HipAdam(torch.optim.Optimizer):
         for i in sel:
             if not grads[i].is_contiguous():
                 grads[i] = ps[i].grad = grads[i].contiguous()
-        n = len(sel)
         tab = t.setdefault("clip", {}).get(sel)       # the pointer tables of what the optimiser itself holds, per set of parameters that have a gradient
         if tab is None:
-            pick = lambda arr, ty: (ty * n)(*[arr[i] for i in sel])
-            P = ctypes.c_void_p
-            tab = t["clip"][sel] = (pick(t["p"], P), pick(t["m"], P), pick(t["v"], P), pick(t["numel"], ctypes.c_int64), pick(t["lr_index"], ctypes.c_int32), P * n)
-        if _lib.ACCESS is not None:                   # (pointer tables: tell a recording capture what this call touches)
-            for i in sel:
-                for x in (ps[i], grads[i], self.state[ps[i]]["exp_avg"], self.state[ps[i]]["exp_avg_sq"]):
-                    _lib.ACCESS.touch(x)
+            pick = lambda arr: [arr[i] or 0 for i in sel]
+            tab = t["clip"][sel] = _lib.host().AdamTable(pick(t["p"]), pick(t["m"]), pick(t["v"]), pick(t["numel"]), pick(t["lr_index"]))
+        if len(sel) != len(grads):
+            grads = [grads[i] for i in sel]
+        if _lib.ACCESS is not None:                   # (tell a recording capture what this call touches)
+            for x in [*grads, *[x for i in sel for x in (ps[i], self.state[ps[i]]["exp_avg"], self.state[ps[i]]["exp_avg_sq"])], self._lr_dev, self._step, self._clip_ws,
+                      self.grad_norm]:
+                _lib.ACCESS.touch(x)
         g0 = self.param_groups[0]
-        with on_device(self.grad_norm):
-            _chk(_lib.lib().vhap_adam_step_clipped(n, tab[0], tab[5](*[grads[i].data_ptr() for i in sel]), tab[1], tab[2], tab[3], tab[4], _p(self._lr_dev), _p(self._step),
-                                                   g0["betas"][0], g0["betas"][1], g0["eps"], self.max_grad_norm, _p(self._clip_ws), self._clip_ws.numel() * 8, _p(self.grad_norm),
-                                                   _lib.CALL_ADAM_STEP_ADVANCED if advanced else (0 if advance else _lib.CALL_ADAM_KEEP_STEP), _stream()),
-                 "vhap_adam_step_clipped")
+        tab.step(grads, self._lr_dev, self._step, g0["betas"][0], g0["betas"][1], g0["eps"], self.max_grad_norm, self._clip_ws, self.grad_norm,
+                 _lib.CALL_ADAM_STEP_ADVANCED if advanced else (0 if advance else _lib.CALL_ADAM_KEEP_STEP))
+        if _lib.ACCESS is not None:
+            _lib.ACCESS.close("vhap_adam_step_clipped")
