@@ -135,6 +135,45 @@ __device__ __forceinline__ void mx_load_raw8(const void* p, long long i, int val
         }
     }
 }
+// Elements k .. k + 7 of a row of `end` that begins at element `row`, in two parts: the load, without a branch around it (a branch there makes the compiler wait at its
+// end, and four such loads in a row cost four round trips instead of one), and, where they are used, what is behind the end: zeros, read again element by element where
+// the eight straddle it.
+template <int DT>
+__device__ __forceinline__ void mx_fetch8(const void* p, long long row, long long k, long long end, MxRaw8<DT>& r) {
+    constexpr int SIZE = DT == VHAP_DTYPE_F32 ? 4 : 2;
+    typedef u32x4 __attribute__((aligned(2))) at2;
+    typedef u32x4 __attribute__((aligned(4))) at4;
+    if (end < 8) return;                                          // (the same for the whole launch)
+    const char* q = static_cast<const char*>(p) + (row + min(k, end - 8)) * SIZE;
+    if constexpr (DT == VHAP_DTYPE_F32) {
+        r.lo = *reinterpret_cast<const at4*>(q);
+        r.hi = *reinterpret_cast<const at4*>(q + 16);
+    } else {
+        r.lo = *reinterpret_cast<const at2*>(q);
+    }
+}
+template <int DT>
+__device__ __forceinline__ void mx_settle8(const void* p, long long row, long long k, long long end, MxRaw8<DT>& r) {
+    if (k + 8 > end) mx_load_raw8<DT>(p, row + k, k >= end ? 0 : (int)(end - k), r);
+}
+
+// the numbers themselves
+template <int DT>
+__device__ __forceinline__ void mx_floats(const MxRaw8<DT>& r, float (&v)[8]) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (DT == VHAP_DTYPE_F32) {
+            v[k] = __uint_as_float(r.lo[k]);
+            v[4 + k] = __uint_as_float(r.hi[k]);
+        } else if constexpr (DT == VHAP_DTYPE_BF16) {
+            v[2 * k] = __uint_as_float(r.lo[k] << 16);
+            v[2 * k + 1] = __uint_as_float(r.lo[k] & 0xffff0000u);
+        } else {
+            v[2 * k] = __half2float(__ushort_as_half((unsigned short)(r.lo[k] & 0xffffu)));
+            v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(r.lo[k] >> 16)));
+        }
+    }
+}
 // their P bf16 fragments (bf16: as they are)
 template <int DT>
 __device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[mx_pieces<DT>()]) {
@@ -142,16 +181,7 @@ __device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[
         out[0] = __builtin_bit_cast(bf16x8, r.lo);
     } else {
         float v[8];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if constexpr (DT == VHAP_DTYPE_F32) {
-                v[k] = __uint_as_float(r.lo[k]);
-                v[4 + k] = __uint_as_float(r.hi[k]);
-            } else {
-                v[2 * k] = __half2float(__ushort_as_half((unsigned short)(r.lo[k] & 0xffffu)));
-                v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(r.lo[k] >> 16)));
-            }
-        }
+        mx_floats<DT>(r, v);
         mx_split8<mx_pieces<DT>()>(v, out);
     }
 }
@@ -159,16 +189,17 @@ __device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[
 __device__ __forceinline__ int mx_left(long long at, long long end) { return at >= end ? 0 : end - at < 8 ? (int)(end - at) : 8; }
 
 // ---- quantise / dequantise: four lanes a block, eight elements a lane (16 or 32 contiguous bytes of x, one dword of codes) ----
-template <int DT>
+// Index: unsigned where rows x blocks x 4 is below 2^31 (a 64-bit division is a hundred instructions), long long beyond.
+template <int DT, typename Index>
 __global__ __launch_bounds__(MX_T) void mx_quantize_kernel(const void* __restrict__ x, long long ldx, long long rows, int K, int Kb, uint8_t* __restrict__ codes,
                                                            uint8_t* __restrict__ scales) {
-    const long long quads = rows * Kb * 4;                       // (a block's four lanes are in one wave, and in or out together)
-    for (long long i = (long long)blockIdx.x * MX_T + threadIdx.x; i < quads; i += (long long)gridDim.x * MX_T) {
-        const long long block = i >> 2;
-        const long long row = block / Kb;
+    const Index quads = (Index)rows * Kb * 4;                    // (a block's four lanes are in one wave, and in or out together)
+    for (Index i = (Index)blockIdx.x * MX_T + threadIdx.x; i < quads; i += (Index)gridDim.x * MX_T) {
+        const Index block = i >> 2;
+        const Index row = block / Kb;
         const int k0 = (int)(block - row * Kb) * 32 + (int)(i & 3) * 8;
         float v[8];
-        vhap_load8(x, row * ldx + k0, DT, mx_left(k0, K), v);
+        vhap_load8(x, (long long)row * ldx + k0, DT, mx_left(k0, K), v);
         unsigned most = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
@@ -195,19 +226,19 @@ __global__ __launch_bounds__(MX_T) void mx_quantize_kernel(const void* __restric
     }
 }
 
-template <int DT>
+template <int DT, typename Index>
 __global__ __launch_bounds__(MX_T) void mx_dequantize_kernel(const MxMatrix w, void* __restrict__ out) {
-    const long long quads = w.rows * w.Kb * 4;
-    for (long long i = (long long)blockIdx.x * MX_T + threadIdx.x; i < quads; i += (long long)gridDim.x * MX_T) {
-        const long long block = i >> 2;
-        const long long row = block / w.Kb;
+    const Index quads = (Index)w.rows * w.Kb * 4;
+    for (Index i = (Index)blockIdx.x * MX_T + threadIdx.x; i < quads; i += (Index)gridDim.x * MX_T) {
+        const Index block = i >> 2;
+        const Index row = block / w.Kb;
         const int k0 = (int)(block - row * w.Kb) * 32 + (int)(i & 3) * 8;
         const unsigned c = reinterpret_cast<const unsigned*>(w.codes)[i];
         const float s = mx_scale(w.scales[block]);
         const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
         const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
         const float v[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
-        vhap_store8(out, row * w.K + k0, DT, mx_left(k0, w.K), v);
+        vhap_store8(out, (long long)row * w.K + k0, DT, mx_left(k0, w.K), v);
     }
 }
 
@@ -264,27 +295,37 @@ __device__ __forceinline__ void mx_decode32(const u32x4& c, float scale, float (
 template <int DT, int MM, int KS>
 __global__ __launch_bounds__(MX_T) void mx_linear_row_kernel(const MxLinear a) {
     const int lane = threadIdx.x & 63, b = lane & 3, r = lane >> 2;
+    __shared__ __attribute__((aligned(16))) float xs[MM][128 * KS];
+    for (int i = threadIdx.x; i < MM * 128 * KS; i += MX_T) {
+        const int m = i / (128 * KS), k = i % (128 * KS);
+        xs[m][k] = m < a.M && k < a.w.K ? mx_one<DT>(a.x, m * a.ldx + k) : 0.f;
+    }
+    __syncthreads();
     float x[MM][KS][32];
 #pragma unroll
     for (int m = 0; m < MM; m++)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+        for (int i = 0; i < 32 * KS; i += 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(&xs[m][128 * (i >> 5) + 32 * b + (i & 31)]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int k0 = 128 * ks + 32 * b + 8 * j;
-                float v[8];
-                vhap_load8(a.x, m * a.ldx + k0, DT, m < a.M ? mx_left(k0, a.w.K) : 0, v);
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[m][ks][8 * j + e] = v[e];
-            }
+            for (int e = 0; e < 4; e++) x[m][i >> 5][(i & 31) + e] = v[e];
+        }
     const long long groups = (a.w.rows + 63) / 64;
-    for (long long g = (long long)blockIdx.x * (MX_T / 64) + (threadIdx.x >> 6); g < groups; g += (long long)gridDim.x * (MX_T / 64)) {
+    for (long long g = (long long)blockIdx.x * (MX_T / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); g < groups; g += (long long)gridDim.x * (MX_T / 64)) {
         u32x4 c[4][KS];
         unsigned s[4][KS];
+        // (the group's place is the same for the wave; inside it 32 bits are enough.  Rows and blocks behind the last: the last one's, as in mx_block)
+        const u32x4* gc = reinterpret_cast<const u32x4*>(a.w.codes) + (size_t)g * 64 * a.w.Kb;
+        const uint8_t* gs = a.w.scales + (size_t)g * 64 * a.w.Kb;
+        const int last = (int)min(63ll, a.w.rows - 1 - g * 64);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) c[t][ks] = mx_block(a.w, g * 64 + 16 * t + r, 4 * ks + b, s[t][ks]);
+            for (int ks = 0; ks < KS; ks++) {
+                const unsigned at = (unsigned)(min(16 * t + r, last) * a.w.Kb + min(4 * ks + b, a.w.Kb - 1));
+                c[t][ks] = gc[at];
+                s[t][ks] = gs[at];
+            }
         const long long n = g * 64 + 16 * b + r;                  // the column that this lane keeps: tile b's
         const float bias = a.bias && n < a.w.rows ? a.bias[n] : 0.f;
         float mine[MM];
@@ -329,15 +370,21 @@ __global__ __launch_bounds__(MX_T) void mx_linear_few_kernel(const MxLinear a) {
     constexpr int P = mx_pieces<DT>();
     const int lane = threadIdx.x & 63, col = lane & 15, q = lane >> 4;
     const int m = col / P, p = col % P;
+    __shared__ __attribute__((aligned(16))) float xs[16 / P][128 * KS];
+    for (int i = threadIdx.x; i < 16 / P * 128 * KS; i += MX_T) {
+        const int row = i / (128 * KS), k = i % (128 * KS);
+        xs[row][k] = row < a.M && k < a.w.K ? mx_one<DT>(a.x, row * a.ldx + k) : 0.f;
+    }
+    __syncthreads();
     bf16x8 xb[KS][4];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int k0 = 128 * ks + 32 * q + 8 * j;
-            float v[8];
+            const float* src = xs[min(m, 16 / P - 1)] + 128 * ks + 32 * q + 8 * j;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(src), hi = *reinterpret_cast<const f32x4*>(src + 4);
+            const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             bf16x8 f[P];
-            vhap_load8(a.x, m * a.ldx + k0, DT, m < a.M ? mx_left(k0, a.w.K) : 0, v);
             mx_split8<P>(v, f);
             xb[ks][j] = f[0];
             if constexpr (P > 1) xb[ks][j] = p == 1 ? f[1] : xb[ks][j];
@@ -428,8 +475,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
         for (int t = 0; t < NT; t++) c[t] = mx_block(a.w, base + 16 * t + (lane >> 2), 4 * ks + (lane & 3), s[t]);
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            const long long m = m0 + 16 * ct + xr;
-            mx_load_raw8<DT>(a.x, m * a.ldx + 128 * ks + xk, m < a.M ? mx_left(128 * ks + xk, a.w.K) : 0, xv[ct]);
+            mx_fetch8<DT>(a.x, min(m0 + 16 * ct + xr, a.M - 1) * a.ldx, 128 * ks + xk, a.w.K, xv[ct]);
         }
     };
     const int from = 4 * (4 * col + q);                                      // (mx_operand, with the loads ahead of their use)
@@ -438,6 +484,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             bf16x8 f[P];
+            mx_settle8<DT>(a.x, min(m0 + 16 * ct + xr, a.M - 1) * a.ldx, 128 * ks + xk, a.w.K, xv[ct]);
             mx_fragments<DT>(xv[ct], f);
 #pragma unroll
             for (int p = 0; p < P; p++) xs[ct][(tid & 15) & 3][p][((tid & 15) >> 2) * 16 + xr] = f[p];
@@ -452,7 +499,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
             w[t][3] = mx_decode8((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c[t].w), sc);
         }
         __syncthreads();
-        if ((ks + 1) * 128 < a.w.K) fetch(ks + 1);
+        fetch(ks + 1);                                                       // (behind the last step: the last elements once more, without a branch)
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -575,19 +622,21 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
         }
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            const long long m = m0 + 16 * ct + col;
-            mx_load_raw8<DT>(a.g, m * a.ldg + n + 8 * q, m < a.M ? mx_left(n + 8 * q, a.w.rows) : 0, ng[ct]);
+            mx_fetch8<DT>(a.g, min(m0 + 16 * ct + col, a.M - 1) * a.ldg, n + 8 * q, a.w.rows, ng[ct]);
         }
     };
-    if (n0 < n1) fetch(n0);
+    fetch(n0);
     for (long long n = n0; n < n1; n += 32) {
         unsigned c[8], s[8];
         bf16x8 gb[CT][P];
 #pragma unroll
         for (int i = 0; i < 8; i++) { c[i] = nc[i]; s[i] = ns[i]; }
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) mx_fragments<DT>(ng[ct], gb[ct]);
-        if (n + 32 < n1) fetch(n + 32);
+        for (int ct = 0; ct < CT; ct++) {
+            mx_settle8<DT>(a.g, min(m0 + 16 * ct + col, a.M - 1) * a.ldg, n + 8 * q, a.w.rows, ng[ct]);
+            mx_fragments<DT>(ng[ct], gb[ct]);
+        }
+        fetch(n + 32);                                            // (behind the last step: rows that are there, without a branch)
 #pragma unroll
         for (int h = 0; h < 4; h++) {                             // elements 2 h and 2 h + 1
             unsigned pk[8];
@@ -662,14 +711,24 @@ __global__ __launch_bounds__(MX_T) void mx_colsum_kernel(const void* __restrict_
     const long long n = ((long long)blockIdx.x * CG + c) * 8;
     const int valid = mx_left(n, N);
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (valid)
+    if (valid == 8) {
 #pragma unroll 4
+        for (long long m = r; m < M; m += RG) {
+            MxRaw8<DT> raw;
+            float x[8];
+            mx_fetch8<DT>(g, m * ldg, n, N, raw);
+            mx_floats<DT>(raw, x);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] += x[e];
+        }
+    } else if (valid) {
         for (long long m = r; m < M; m += RG) {
             float x[8];
             vhap_load8(g, m * ldg + n, DT, valid, x);
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] += x[e];
         }
+    }
     if constexpr (RG > 1) {
 #pragma unroll
         for (int e = 0; e < 8; e++) red[r][c][e] = v[e];
@@ -863,7 +922,7 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
     const long long N = a.w.rows;
     const int ks = (a.w.K + 127) / 128;
     if (a.M <= 2 && ks <= (a.M == 1 ? 4 : 2)) {
-        const int grid = mx_grid((N + 63) / 64 * 64, 2048);
+        const int grid = mx_grid((N + 63) / 64 * 64, 1024);
         if (a.M == 2) {
             if (ks == 1) mx_linear_row_kernel<DT, 2, 1><<<grid, MX_T, 0, st>>>(a);
             else mx_linear_row_kernel<DT, 2, 2><<<grid, MX_T, 0, st>>>(a);
@@ -924,7 +983,9 @@ extern "C" int vhap_mx4_quantize(const void* x, int dtype, long long ldx, long l
     if (rows == 0) return VHAP_OK;
     if (!x || !codes || !scales) return VHAP_E_NULLPTR;
     const int Kb = mx_kb(K);
-    MX_BY_TYPE(dtype, (mx_quantize_kernel<DT><<<mx_grid(rows * Kb * 4, 16384), MX_T, 0, vhap_stream(stream)>>>(x, ldx, rows, K, Kb, codes, scales)));
+    const int grid = mx_grid(rows * Kb * 4, 16384);
+    if (rows * Kb * 4 + 16384ll * MX_T < (1ll << 31)) MX_BY_TYPE(dtype, (mx_quantize_kernel<DT, unsigned><<<grid, MX_T, 0, vhap_stream(stream)>>>(x, ldx, rows, K, Kb, codes, scales)))
+    else MX_BY_TYPE(dtype, (mx_quantize_kernel<DT, long long><<<grid, MX_T, 0, vhap_stream(stream)>>>(x, ldx, rows, K, Kb, codes, scales)));
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
 }
@@ -935,7 +996,9 @@ extern "C" int vhap_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, 
     if (rows == 0) return VHAP_OK;
     if (!out || !codes || !scales) return VHAP_E_NULLPTR;
     const MxMatrix w{codes, scales, rows, K, mx_kb(K)};
-    MX_BY_TYPE(dtype, (mx_dequantize_kernel<DT><<<mx_grid(rows * w.Kb * 4, 16384), MX_T, 0, vhap_stream(stream)>>>(w, out)));
+    const int grid = mx_grid(rows * w.Kb * 4, 16384);
+    if (rows * w.Kb * 4 + 16384ll * MX_T < (1ll << 31)) MX_BY_TYPE(dtype, (mx_dequantize_kernel<DT, unsigned><<<grid, MX_T, 0, vhap_stream(stream)>>>(w, out)))
+    else MX_BY_TYPE(dtype, (mx_dequantize_kernel<DT, long long><<<grid, MX_T, 0, vhap_stream(stream)>>>(w, out)));
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
 }
@@ -977,12 +1040,12 @@ extern "C" int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ld
 
 extern "C" int vhap_mx4_column_sums(const void* g, int dtype, long long ldg, long long M, long long N, float* out, vhap_stream_t stream) {
     VHAP_ENTER();
-    if (!mx_dims(M, 1) || !mx_dims(N, 1) || !mx_dt(dtype) || ldg < 0 || N / 64 >= (1ll << 31) - 1) return VHAP_E_BADDIM;
+    if (!mx_dims(M, 1) || !mx_dims(N, 1) || !mx_dt(dtype) || ldg < 0 || N / 32 >= (1ll << 31) - 1) return VHAP_E_BADDIM;
     if (N == 0) return VHAP_OK;
     if (!out || (M > 0 && !g)) return VHAP_E_NULLPTR;
-    // few rows: every thread sums its own columns; from eight rows on 32 threads share them (64 columns a block)
+    // few rows: every thread sums its own columns; from eight rows on 64 threads share them (32 columns a block)
     if (M < 8) MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 1><<<vhap_cdiv(N, 8 * MX_T), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)))
-    else MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 32><<<vhap_cdiv(N, 8 * MX_T / 32), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)));
+    else MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 64><<<vhap_cdiv(N, 8 * MX_T / 64), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)));
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
 }
