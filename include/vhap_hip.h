@@ -908,7 +908,7 @@ int vhap_nhwc_add(const float* a, const float* b, const float* c, long long n, f
  * Microscaled 4-bit floating point (vhap_amd/csrc/mx.hip; host side: vhap_amd/mx.py).  A row of K numbers is Kb = ceil(K / 32) blocks of 32 codes of E2M1
  * (+-{0, 0.5, 1, 1.5, 2, 3, 4, 6}; two a byte, the even element in the low half) and one byte b a block, the power of two 2^(b - 127) its codes are
  * multiplied with; b = 255: the block is NaN.  codes [rows, 16 Kb] (16-byte aligned), scales [rows, Kb], both contiguous.  Codes behind K in the last block
- * are written as zero and read as nothing.  dtype: VHAP_DTYPE_* of the floating-point operand.  Row strides (ldx, ldg) in elements; rows < 2^40, K <= 2^24.
+ * are written as zero and read as nothing.  An element past float32's range (b = 253 or 254; quantize makes none) counts as infinite.  dtype: VHAP_DTYPE_* of the floating-point operand.  Row strides (ldx, ldg) in elements; rows < 2^40, K <= 2^24.
  *   vhap_mx4_quantize: x [rows, K].  b from the block's largest magnitude (exponent - 2: the largest code in [4, 8), 6 where it would be more), codes to nearest,
  *     halves to the even code; a block with a NaN or an infinity becomes NaN.
  *   vhap_mx4_dequantize: out [rows, K] contiguous (float32 and bfloat16 hold every value exactly; float16 rounds, and overflows above 65504).

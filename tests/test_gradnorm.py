@@ -380,3 +380,37 @@ def test_clipped_adam_counter_flags_and_capture():
             ob.step()
             torch.cuda.synchronize()
             assert torch.equal(a.detach(), b.detach()) and torch.equal(oa.grad_norm, ob.grad_norm) and int(oa.step_count) == k + 1
+
+
+def test_a_negated_view_is_refused():
+    """.imag of a conjugated tensor is real, dense and holds the opposite of what its memory does"""
+    x = torch.randn(8, dtype=torch.complex64).conj().imag
+    assert x.is_neg()
+    for call in (lambda: NV.grad_norm([x]), lambda: NV.clip_by_global_norm([x], 1.0), lambda: NV.clip_by_global_norm([torch.ones(8)], 1.0, out=[x])):
+        with pytest.raises((TypeError, RuntimeError)):
+            call()
+    with pytest.raises(TypeError, match="negated"):
+        NV.grad_norm([x])
+
+
+@pytest.mark.gpu
+def test_strided_results_side_by_side_and_overlapping():
+    buf = randn((40, 60), 1, scale=3.0)
+    src = buf.clone()
+    views = [buf[:, :25], buf[:, 25:59], buf[:, 59:]]                            # columns of one matrix: the norm is the matrix's
+    _, norm = NV.clip_by_global_norm(views, 1.0, out=views)
+    want = norm64([src], 2)
+    assert near_norm(float(norm), want)
+    check_clipped(buf, src, coefficient(want, 1.0))
+    g = [randn((40, 30), 2), randn((40, 30), 3)]
+    square = torch.empty(30, 40, device="cuda")
+    for out in ([buf[:, :30], buf[:, 29:59]], [buf[:, :30], buf[::1, :30]], [buf[:, 30:], buf[:, :31][:, 1:]], [square.t(), square.view(40, 30)],
+                [buf[:, :30], buf.view(-1)[45:45 + 1200].view(40, 30)]):
+        keep = buf.clone()
+        with pytest.raises(ValueError, match="overlap|twice"):
+            NV.clip_by_global_norm(g, 1.0, out=out)
+        assert torch.equal(buf, keep)
+    out = [buf[:, 30:], buf[:, :30]]                                             # in the other order in memory
+    _, norm = NV.clip_by_global_norm(g, 1.0, out=out)
+    for o, x in zip(out, g):
+        check_clipped(o, x, coefficient(norm64(g, 2), 1.0))

@@ -403,3 +403,83 @@ def test_a_code_is_fitted_in_a_4_bit_basis():
         opt.step()
         n = float(code.grad.double().norm())
         assert abs(float(opt.grad_norm) - n) <= 1.01 * 2.0 ** -24 * n
+
+
+def test_a_negated_view_is_refused():
+    x = torch.randn(4, 40, dtype=torch.complex64).conj().imag
+    w = random_mx(4, 40, 1, "cpu")
+    for call in (lambda: mx.quantize(x), lambda: mx.linear(x, w), lambda: mx.linear(torch.ones(4, 40), w, x[:, 0])):
+        with pytest.raises((TypeError, RuntimeError)):
+            call()
+    with pytest.raises(TypeError, match="negated"):
+        mx.quantize(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m", [1, 4, 20])
+def test_linear_with_scales_at_the_ends(m, dtype):
+    """the smallest scales (elements down to 2^-128, subnormal in bf16 and fp32) against large numbers, the largest finite ones against small numbers"""
+    for lo, hi, times in ((0, 4, 2.0 ** 110), (248, 253, 2.0 ** -90)):
+        w = random_mx(70, 200, 1, lo=lo, hi=hi)
+        W = values64(w)
+        x, g = (randn((m, 200), 2) * times).to(dtype), (randn((m, 70), 3) * times).to(dtype)
+        X, G, P = x.cpu().double(), g.cpu().double(), PIECES[dtype]
+        check_sum(mx.linear(x, w), X @ W.t(), X.abs() @ W.abs().t(), 200 * P, dtype)
+        check_sum(mx.linear_input_grad(g, w), G @ W, G.abs() @ W.abs(), 70 * P + 1024, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lo,hi", [((0, 3), (252, 255)), ((0, 255), (127, 128)), ((0, 1), (0, 1))])
+def test_matmul_with_scales_at_the_ends(lo, hi):
+    a, b = random_mx(40, 200, 1, lo=lo[0], hi=lo[1]), random_mx(70, 200, 2, lo=hi[0], hi=hi[1])
+    A, B = values64(a), values64(b)
+    want, mags = A @ B.t(), A.abs() @ B.abs().t()
+    got = mx.matmul(a, b).cpu().double()
+    fits = mags < 2.0 ** 126
+    off = (got - want).abs()
+    assert bool((off <= (204 * 2.0 ** -23) * mags + 2.0 ** -126)[fits].all()) and bool(fits.any())       # (a sum below the normal numbers may be cut off)
+
+
+@pytest.mark.gpu
+def test_gradients_over_many_rows():
+    """more tiles of rows than a grid's second or third axis holds"""
+    m = 64 * 65536 + 1
+    w = random_mx(8, 33, 1)
+    g = randn((64, 8), 2, torch.bfloat16).repeat(65537, 1)[:m]
+    dx = mx.linear_input_grad(g, w)
+    for at in (0, 64 * 40000, m - 65):
+        assert torch.equal(dx[at:at + 64], mx.linear_input_grad(g[at:at + 64], w))
+    L, n = _lib.lib(), 2 ** 29 + 5                                               # and as many columns
+    g = torch.arange(n, device="cuda").remainder(251).to(torch.bfloat16)
+    out = torch.empty(n, dtype=torch.float32, device="cuda")
+    assert L.vhap_mx4_column_sums(g.data_ptr(), 1, 0, 8, n, out.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, g.float() * 8)                                       # (the same row eight times)
+
+
+@pytest.mark.gpu
+def test_a_captured_backward():
+    """forward and backward in a capture, replayed against the eager ones; and refused while an eager graph of the same leaf is alive"""
+    w, bias = random_mx(300, 90, 1), randn((300,), 2).requires_grad_()
+    x, g = randn((5, 90), 3).requires_grad_(), randn((5, 300), 4)
+    y = mx.linear(x, w, bias)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="alive"):
+        with torch.cuda.graph(graph):
+            mx.linear(x, w, bias)
+    del y
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = mx.linear(x, w, bias)
+        dx, db = torch.autograd.grad(y, (x, bias), g)
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(randn((5, 90), 10 + k))
+            g.copy_(randn((5, 300), 20 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        x1 = x.detach().clone().requires_grad_()
+        y1 = mx.linear(x1, w, bias.detach())
+        assert torch.equal(y.detach(), y1.detach()) and torch.equal(dx, torch.autograd.grad(y1, x1, g)[0])
+        assert torch.equal(db, torch.autograd.grad(mx.linear(x1, w, b1 := bias.detach().clone().requires_grad_()), b1, g)[0])

@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -58,6 +59,10 @@ int dtype_code(at::ScalarType t) {
 
 vhap_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
+void plain(const Tensor& t, const char* what) {
+    if (t.is_neg()) throw py::type_error(text(what, ": a view whose elements are negated when they are read (resolve_neg() it first)"));
+}
+
 void on_hip(const Tensor& t, const char* what) {
     if (!t.is_cuda()) throw std::runtime_error(text(what, ": tensors on a HIP device (no CPU fallback)"));
 }
@@ -83,6 +88,7 @@ List gradients(py::handle given, const char* what) {
         const Tensor& t = THPVariable_Unpack(items[i]);
         if (t.layout() != at::kStrided || dtype_code(t.scalar_type()) < 0)
             throw py::type_error(text(what, ": dense float32, bfloat16 or float16 tensors, got ", t.scalar_type(), " (", t.layout(), ")"));
+        plain(t, what);
         on_hip(t, what);
         if (i > 0 && t.device() != l[0].device()) throw py::value_error(text(what, ": tensors on one device, got ", l[0].device(), " and ", t.device()));
         l.t.push_back(&t);
@@ -132,6 +138,30 @@ Tensor grad_norm(py::handle given, int kind) {
     return norm;
 }
 
+// Where a result lies: bytes [lo, hi), as runs of at most `run` bytes, `step` apart (the axis of the largest stride; step 0: a single run).
+struct Place {
+    uintptr_t lo, hi, step, run;
+    explicit Place(const Tensor& t) {
+        const int64_t size = (int64_t)t.element_size();
+        int64_t outer = -1, all = 0;
+        for (int64_t d = 0; d < t.dim(); d++) {
+            all += (t.size(d) - 1) * t.stride(d);
+            if (t.size(d) > 1 && (outer < 0 || t.stride(d) > t.stride(outer))) outer = d;
+        }
+        lo = (uintptr_t)t.data_ptr();
+        hi = lo + (all + 1) * size;
+        step = outer < 0 ? 0 : t.stride(outer) * size;
+        run = outer < 0 ? size : hi - lo - (t.size(outer) - 1) * step;
+    }
+    // nothing in common, as far as can be seen: apart, or (columns of one matrix) runs in different places of the same step
+    bool apart(const Place& b) const {
+        if (hi <= b.lo || b.hi <= lo) return true;
+        if (step == 0 || step != b.step) return false;
+        const uintptr_t to = b.lo >= lo ? (b.lo - lo) % step : (step - (lo - b.lo) % step) % step;
+        return to >= run && to + b.run <= step;
+    }
+};
+
 // -> (results, norm); `out` None: new tensors
 py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
     at::NoGradGuard no_grad;
@@ -162,7 +192,6 @@ py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
     // the kernels walk memory in order: a pair that is dense with the same strides is taken as it stands, anything else goes through contiguous copies
     Table t(gs.size());
     std::vector<std::pair<Tensor, Tensor>> back;
-    std::set<std::tuple<const void*, std::vector<int64_t>, std::vector<int64_t>>> strided;
     std::vector<Tensor> keep;
     for (size_t i = 0; i < gs.size(); i++) {
         const Tensor &g = gs[i], &o = outs[i];
@@ -172,11 +201,24 @@ py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
         }
         for (int64_t d = 0; d < o.dim(); d++)
             if (o.stride(d) == 0 && o.size(d) > 1) throw py::value_error(text(what, ": a result whose elements share memory (an expanded tensor)"));
-        if (!strided.emplace(o.data_ptr(), o.sizes().vec(), o.strides().vec()).second) throw py::value_error("clipping: the same tensor twice in the list");
         const Tensor c = g.contiguous(), r = at::empty(c.sizes(), c.options());
         t.add(c, &r);
         keep.push_back(c);
         back.emplace_back(o, r);
+    }
+    if (!back.empty()) {                      // (dense ones among themselves: vhap_grad_clip sees to it)
+        std::vector<std::pair<Place, size_t>> at;
+        for (size_t i = 0; i < outs.size(); i++)
+            if (outs[i].numel() > 0) at.emplace_back(Place(outs[i]), i);
+        for (auto& b : back) {
+            if (b.first.numel() == 0) continue;
+            const Place mine(b.first);
+            for (auto& x : at)
+                if (!b.first.is_same(outs[x.second]) && !mine.apart(x.first)) throw py::value_error("clipping: a strided result overlaps another result in memory");
+        }
+        std::set<const void*> once;
+        for (auto& b : back)
+            if (!once.insert(b.first.unsafeGetTensorImpl()).second) throw py::value_error("clipping: the same tensor twice in the list");
     }
     const size_t bytes = api.norm_bytes((int)gs.size());
     const Tensor ws = workspace(bytes, gs[0]), norm = at::empty({}, gs[0].options().dtype(at::kFloat));
@@ -239,6 +281,7 @@ std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
 void floats(const Tensor& t, const char* what) {
     if (t.layout() != at::kStrided || dtype_code(t.scalar_type()) < 0)
         throw py::type_error(text(what, ": a float32, bfloat16 or float16 tensor, got ", t.scalar_type(), " (", t.layout(), ")"));
+    plain(t, what);
 }
 
 void pair_ok(const Tensor& x, const Tensor& codes, int64_t n, int64_t N, int64_t K, const char* what) {
@@ -251,6 +294,7 @@ void pair_ok(const Tensor& x, const Tensor& codes, int64_t n, int64_t N, int64_t
 void bias_ok(const std::optional<Tensor>& bias, int64_t N, c10::Device device, const char* what) {
     if (!bias) return;
     if (bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != N) throw py::value_error(text(what, ": a float32 bias of ", N, " elements"));
+    plain(*bias, what);
     if (bias->device() != device) throw py::value_error(text(what, ": the bias on ", device, ", got ", bias->device()));
 }
 
@@ -329,12 +373,27 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
     }
 };
 
+// A leaf's gradient node keeps the stream it was made on for as long as any graph holds it.  One made outside a capture would make the captured backward wait for that
+// stream, which a capture does not survive (the runtime ends the process): said here, while it can be.
+void capture_ok(const Tensor& t, const char* what) {
+    if (!t.requires_grad() || !t.is_leaf()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) return;
+    const auto made_on = node->stream();
+    if (made_on && made_on->id() != c10::hip::getCurrentHIPStream(t.device().index()).id())
+        throw std::runtime_error(text(what, ": in a stream capture, while a graph of the same leaf made on another stream is alive (delete its results first)"));
+}
+
 Tensor linear(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t N, int64_t K, const std::optional<Tensor>& bias) {
     pair_ok(x, codes, K, N, K, "linear");
     bias_ok(bias, N, x.device(), "linear");
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || (bias && bias->requires_grad()))) {
         at::NoGradGuard no_grad;
         return run_linear(x, codes, scales, N, K, bias ? *bias : Tensor());
+    }
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+        capture_ok(x, "linear");
+        if (bias) capture_ok(*bias, "linear");
     }
     return MxLinear::apply(x, codes, scales, N, K, bias);
 }

@@ -28,6 +28,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));      // (HIP's uint4 holds a union: arrays of it end up in scratch memory)
 
 constexpr int MX_T = 256;
+constexpr long long MX_MOST_BLOCKS = (1ll << 24) - 1;            // a grid holds fewer than 2^32 threads
 
 struct MxMatrix {
     const uint8_t* codes;     // [rows, 16 Kb]
@@ -530,7 +531,12 @@ struct MxInputGrad {
     MxMatrix w;               // [N, K]
     float* part;              // [splits, M, 128 ktiles]
     int ktiles;
+    unsigned splits;
     long long steps_per_wave; // of 32 rows of W
+    // the grid has one axis (a grid's second and third end at 65535): splits fastest, then tiles of K, then tiles of M
+    __device__ __forceinline__ unsigned split() const { return blockIdx.x % splits; }
+    __device__ __forceinline__ int kt() const { return (int)(blockIdx.x / splits % (unsigned)ktiles); }
+    __device__ __forceinline__ unsigned mt() const { return blockIdx.x / splits / (unsigned)ktiles; }
 };
 
 // One or two rows of g: per 16 rows of W a lane decodes one block of 32 (four lanes a row) and adds it, times g, to its 32 sums -- 16 conversions and 32 M
@@ -539,13 +545,14 @@ template <int DT, int MM>
 __global__ __launch_bounds__(MX_T) void mx_input_grad_few_kernel(const MxInputGrad a) {
     __shared__ float red[MX_T / 64][MM][128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = lane & 3, r = lane >> 2;
-    const int blk = 4 * blockIdx.y + b;
+    const int kt = a.kt(), blk = 4 * kt + b;
+    const unsigned split = a.split();
     float acc[MM][32];
 #pragma unroll
     for (int m = 0; m < MM; m++)
 #pragma unroll
         for (int e = 0; e < 32; e++) acc[m][e] = 0.f;
-    const long long n0 = ((long long)blockIdx.x * (MX_T / 64) + wave) * a.steps_per_wave * 32;
+    const long long n0 = ((long long)split * (MX_T / 64) + wave) * a.steps_per_wave * 32;
     const long long n1 = min(n0 + a.steps_per_wave * 32, a.w.rows);
     for (long long n = n0; n < n1; n += 32) {
         u32x4 c[2];
@@ -589,7 +596,7 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_few_kernel(const MxInputGr
     __syncthreads();
     for (int i = threadIdx.x; i < MM * 128; i += MX_T) {
         const int m = i >> 7, k = i & 127;
-        if (m < a.M) a.part[((size_t)blockIdx.x * a.M + m) * (128 * a.ktiles) + 128 * blockIdx.y + k] = (red[0][m][k] + red[1][m][k]) + (red[2][m][k] + red[3][m][k]);
+        if (m < a.M) a.part[((size_t)split * a.M + m) * (128 * a.ktiles) + 128 * kt + k] = (red[0][m][k] + red[1][m][k]) + (red[2][m][k] + red[3][m][k]);
     }
 }
 
@@ -601,15 +608,16 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
     constexpr int P = mx_pieces<DT>();
     __shared__ f32x4 red[8][CT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q = lane >> 4;
-    const int kt = blockIdx.y;
-    const long long m0 = (long long)blockIdx.z * 16 * CT;
+    const int kt = a.kt();
+    const unsigned split = a.split();
+    const long long m0 = (long long)a.mt() * 16 * CT;
     const int blk = 4 * kt + (col >> 2);                          // the block that this lane's eight elements lie in
     f32x4 acc[8][CT];
 #pragma unroll
     for (int k = 0; k < 8; k++)
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) acc[k][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const long long n0 = ((long long)blockIdx.x * (MX_T / 64) + wave) * a.steps_per_wave * 32;
+    const long long n0 = ((long long)split * (MX_T / 64) + wave) * a.steps_per_wave * 32;
     const long long n1 = min(n0 + a.steps_per_wave * 32, a.w.rows);
     unsigned nc[8], ns[8];                                        // the next 32 rows, on their way while these are multiplied
     MxRaw8<DT> ng[CT];
@@ -674,7 +682,7 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
         const int k = i & 127, mm = i >> 7;
         const long long m = m0 + mm;
         const int row = k >> 3;
-        if (m < a.M) a.part[((size_t)blockIdx.x * a.M + m) * (128 * a.ktiles) + 128 * kt + k] = red[k & 7][mm >> 4][(row >> 2) * 16 + (mm & 15)][row & 3];
+        if (m < a.M) a.part[((size_t)split * a.M + m) * (128 * a.ktiles) + 128 * kt + k] = red[k & 7][mm >> 4][(row >> 2) * 16 + (mm & 15)][row & 3];
     }
 }
 
@@ -683,22 +691,24 @@ template <int DT, int EL, int SG>
 __global__ __launch_bounds__(EL * SG) void mx_join_kernel(const float* __restrict__ part, int splits, long long M, int K, int Kp, void* __restrict__ dx, int accumulate) {
     __shared__ float red[SG][EL];
     const int e = threadIdx.x % EL, sg = threadIdx.x / EL;
-    const long long i = (long long)blockIdx.x * EL + e;
-    const long long m = i / K;
-    const int k = (int)(i - m * K);
-    float v = 0.f;
-    if (m < M) {
-        const float* p = part + m * Kp + k;
+    for (long long i0 = (long long)blockIdx.x * EL; i0 < M * K; i0 += (long long)gridDim.x * EL) {
+        const long long i = i0 + e, m = i / K;
+        const int k = (int)(i - m * K);
+        float v = 0.f;
+        if (m < M) {
+            const float* p = part + m * Kp + k;
 #pragma unroll 8
-        for (int s = sg; s < splits; s += SG) v += p[(size_t)s * M * Kp];
-    }
-    red[sg][e] = v;
-    __syncthreads();
-    if (sg == 0 && m < M) {
+            for (int s = sg; s < splits; s += SG) v += p[(size_t)s * M * Kp];
+        }
+        red[sg][e] = v;
+        __syncthreads();
+        if (sg == 0 && m < M) {
 #pragma unroll 8
-        for (int j = 1; j < SG; j++) v += red[j][e];
-        if (DT == VHAP_DTYPE_F32 && accumulate) v = static_cast<float*>(dx)[i] + v;
-        mx_put<DT>(dx, i, v);
+            for (int j = 1; j < SG; j++) v += red[j][e];
+            if (DT == VHAP_DTYPE_F32 && accumulate) v = static_cast<float*>(dx)[i] + v;
+            mx_put<DT>(dx, i, v);
+        }
+        __syncthreads();
     }
 }
 
@@ -877,7 +887,7 @@ __global__ __launch_bounds__(MX_T) void mx_matmul_kernel(const MxMatmul a, long 
 template <int DT, int BM, int BN>
 int mx_matmul_launch(const MxMatmul& a, hipStream_t st) {
     const long long mtiles = (a.a.rows + BM - 1) / BM, tiles = mtiles * ((a.b.rows + BN - 1) / BN);
-    if (tiles >= (1ll << 31)) return VHAP_E_BADDIM;
+    if (tiles > MX_MOST_BLOCKS) return VHAP_E_BADDIM;
     if (a.b.K % (32 * MM_Q) == 0) mx_matmul_kernel<DT, BM, BN, true><<<(int)tiles, MX_T, 0, st>>>(a, mtiles);
     else mx_matmul_kernel<DT, BM, BN, false><<<(int)tiles, MX_T, 0, st>>>(a, mtiles);
     VHAP_LAUNCH_CHECK();
@@ -945,7 +955,7 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
     // 256 rows of W a block, or 128 where that leaves fewer than two blocks a CU
     const bool wide = mtiles * ((N + 255) / 256) >= 512;
     const long long tiles = mtiles * ((N + (wide ? 255 : 127)) / (wide ? 256 : 128));
-    if (tiles >= (1ll << 31)) return VHAP_E_BADDIM;
+    if (tiles > MX_MOST_BLOCKS) return VHAP_E_BADDIM;
 #define MX_LINEAR(NT, CT) mx_linear_kernel<DT, NT, CT><<<(int)tiles, MX_T, 0, st>>>(a, mtiles)
     if (wide) {
         if (ct == 1) MX_LINEAR(4, 1); else if (ct == 2) MX_LINEAR(4, 2); else MX_LINEAR(4, 4);
@@ -959,7 +969,7 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
 
 template <int DT>
 int mx_input_grad_launch(const MxInputGrad& a, const GradPlan& p, void* dx, int accumulate, hipStream_t st) {
-    const dim3 grid((unsigned)p.splits, p.ktiles, (unsigned)p.mtiles);
+    const unsigned grid = (unsigned)(p.splits * p.ktiles * p.mtiles);
     if (p.few) {
         if (a.M == 1) mx_input_grad_few_kernel<DT, 1><<<grid, MX_T, 0, st>>>(a);
         else mx_input_grad_few_kernel<DT, 2><<<grid, MX_T, 0, st>>>(a);
@@ -969,8 +979,8 @@ int mx_input_grad_launch(const MxInputGrad& a, const GradPlan& p, void* dx, int 
     VHAP_LAUNCH_CHECK();
     const long long n = a.M * a.w.K;
     // many splits of few elements: 64 threads an element; else four
-    if (p.splits > 64) mx_join_kernel<DT, 16, 64><<<vhap_cdiv(n, 16), 1024, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
-    else mx_join_kernel<DT, 64, 4><<<vhap_cdiv(n, 64), 256, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
+    if (p.splits > 64) mx_join_kernel<DT, 16, 64><<<(int)std::min((n + 15) / 16, 1ll << 20), 1024, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
+    else mx_join_kernel<DT, 64, 4><<<(int)std::min((n + 63) / 64, 1ll << 20), 256, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
 }
@@ -1030,9 +1040,9 @@ extern "C" int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ld
     if (M == 0) return VHAP_OK;
     if (!g || !codes || !scales || !dx || !workspace) return VHAP_E_NULLPTR;
     const GradPlan p = mx_grad_plan(M, N, K);
-    if (p.ktiles > 65535 || p.mtiles > 65535 || M * K / 16 >= (1ll << 31) - 1) return VHAP_E_BADDIM;
+    if (p.splits * p.ktiles > MX_MOST_BLOCKS / p.mtiles) return VHAP_E_BADDIM;
     if (workspace_bytes < vhap_mx4_linear_input_grad_workspace_bytes(M, N, K)) return VHAP_E_WORKSPACE;
-    const MxInputGrad a{g, ldg, M, {codes, scales, N, K, mx_kb(K)}, static_cast<float*>(workspace), p.ktiles, p.steps_per_wave};
+    const MxInputGrad a{g, ldg, M, {codes, scales, N, K, mx_kb(K)}, static_cast<float*>(workspace), p.ktiles, (unsigned)p.splits, p.steps_per_wave};
     int rc = VHAP_OK;
     MX_BY_TYPE(dtype, rc = mx_input_grad_launch<DT>(a, p, dx, accumulate, vhap_stream(stream)));
     return rc;
@@ -1040,11 +1050,11 @@ extern "C" int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ld
 
 extern "C" int vhap_mx4_column_sums(const void* g, int dtype, long long ldg, long long M, long long N, float* out, vhap_stream_t stream) {
     VHAP_ENTER();
-    if (!mx_dims(M, 1) || !mx_dims(N, 1) || !mx_dt(dtype) || ldg < 0 || N / 32 >= (1ll << 31) - 1) return VHAP_E_BADDIM;
+    if (!mx_dims(M, 1) || !mx_dims(N, 1) || !mx_dt(dtype) || ldg < 0 || N / (8 * MX_T) >= MX_MOST_BLOCKS) return VHAP_E_BADDIM;
     if (N == 0) return VHAP_OK;
     if (!out || (M > 0 && !g)) return VHAP_E_NULLPTR;
-    // few rows: every thread sums its own columns; from eight rows on 64 threads share them (32 columns a block)
-    if (M < 8) MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 1><<<vhap_cdiv(N, 8 * MX_T), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)))
+    // few rows: every thread sums its own columns; from eight rows on 64 threads share them (32 columns a block, as long as a grid has room for that)
+    if (M < 8 || N / 32 >= MX_MOST_BLOCKS) MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 1><<<vhap_cdiv(N, 8 * MX_T), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)))
     else MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 64><<<vhap_cdiv(N, 8 * MX_T / 64), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)));
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;

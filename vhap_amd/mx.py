@@ -23,7 +23,8 @@ _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 class MXTensor:
     """[..., K] numbers in 4 bits: `codes` uint8 [..., 16 Kb], `scales` uint8 [..., Kb], Kb = ceil(K / 32), both contiguous.  Codes behind K are not read as
-    numbers.  `shape` is that of the numbers."""
+    numbers.  `shape` is that of the numbers.  An element past float32's range (its block's byte 253 or 254: quantize makes none) counts as infinite, and what it
+    enters is not finite."""
 
     def __init__(self, codes, scales, shape):
         shape = torch.Size(int(n) for n in shape)
@@ -120,7 +121,9 @@ def quantize_host(x):
 
 def linear(x, w, bias=None):
     """y [..., N] = x [..., K] w^T (+ bias): w an MXTensor [N, K], x float32 / bfloat16 / float16, bias float32 [N]; y in x's type.  The products are exact,
-    the sums are float32 in a fixed order, y is rounded once.  Gradients flow to x and bias (once: not twice differentiable)."""
+    the sums are float32 in a fixed order, y is rounded once (float32 numbers below 2^-117 lose their last bits, those below 2^-126 may count as 0).  Gradients
+    flow to x and bias (once: not twice differentiable).  In a stream capture, a differentiable call is refused while a graph of the same leaf made on another
+    stream is alive: its captured backward would end the process."""
     N, K = _matrix(w, "linear")
     return _lib.host().linear(x, w.codes, w.scales, N, K, bias)
 
