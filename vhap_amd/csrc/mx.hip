@@ -529,7 +529,9 @@ struct MxInputGrad {
     const void* g;            // [M, N], rows ldg apart
     long long ldg, M;
     MxMatrix w;               // [N, K]
-    float* part;              // [splits, M, 128 ktiles]
+    float* part;              // [splits, M, 128 ktiles], for more than one split or one or two rows
+    void* dx;
+    int accumulate;
     int ktiles;
     unsigned splits;
     long long steps_per_wave; // of 32 rows of W
@@ -605,8 +607,8 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_few_kernel(const MxInputGr
 // matrix instruction over 32 rows.
 template <int DT, int CT>
 __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a) {
-    constexpr int P = mx_pieces<DT>();
-    __shared__ f32x4 red[8][CT][64];
+    constexpr int P = mx_pieces<DT>(), WAVES = MX_T / 64;
+    __shared__ f32x4 red[CT > 1 ? 2 : 1][WAVES][4][2][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q = lane >> 4;
     const int kt = a.kt();
     const unsigned split = a.split();
@@ -617,7 +619,7 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
     for (int k = 0; k < 8; k++)
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) acc[k][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const long long n0 = ((long long)split * (MX_T / 64) + wave) * a.steps_per_wave * 32;
+    const long long n0 = ((long long)split * WAVES + wave) * a.steps_per_wave * 32;
     const long long n1 = min(n0 + a.steps_per_wave * 32, a.w.rows);
     unsigned nc[8], ns[8];                                        // the next 32 rows, on their way while these are multiplied
     MxRaw8<DT> ng[CT];
@@ -669,44 +671,62 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
                 }
         }
     }
-    for (int w = 0; w < MX_T / 64; w++) {                         // the four waves, in order
-        if (wave == w)
+    // The four waves' sums, in order: 16 rows of g at a time through LDS.  A lane holds, of row `col`, the 32 consecutive elements of K from 32 q on (element 8 i + e in
+    // register i of acc[e]); wave w joins and stores the eight of i = w.
 #pragma unroll
-            for (int k = 0; k < 8; k++)
+    for (int ct = 0; ct < CT; ct++) {
+        auto buf = red[CT > 1 ? ct & 1 : 0];                      // (two by turns: one barrier a round)
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) red[k][ct][lane] = w == 0 ? acc[k][ct] : red[k][ct][lane] + acc[k][ct];
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) buf[wave][i][h][lane] = f32x4{acc[4 * h][ct][i], acc[4 * h + 1][ct][i], acc[4 * h + 2][ct][i], acc[4 * h + 3][ct][i]};
         __syncthreads();
-    }
-    // element k of row m: instruction row (k % 128) / 8 -> lane group and register, column m
-    for (int i = threadIdx.x; i < 16 * CT * 128; i += MX_T) {
-        const int k = i & 127, mm = i >> 7;
-        const long long m = m0 + mm;
-        const int row = k >> 3;
-        if (m < a.M) a.part[((size_t)split * a.M + m) * (128 * a.ktiles) + 128 * kt + k] = red[k & 7][mm >> 4][(row >> 2) * 16 + (mm & 15)][row & 3];
+        f32x4 v[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            v[h] = buf[0][wave][h][lane];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) v[h] += buf[w][wave][h][lane];
+        }
+        const long long m = m0 + 16 * ct + col;
+        const int k = 128 * kt + 32 * q + 8 * wave;
+        if (m < a.M && a.splits > 1) {
+            f32x4* out = reinterpret_cast<f32x4*>(a.part + ((size_t)split * a.M + m) * (128 * a.ktiles) + k);
+            out[0] = v[0];
+            out[1] = v[1];
+        } else if (m < a.M) {
+            const int valid = mx_left(k, a.w.K);
+            float o[8], was[8];
+            if (DT == VHAP_DTYPE_F32 && a.accumulate) vhap_load8(a.dx, m * a.w.K + k, DT, valid, was);
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = DT == VHAP_DTYPE_F32 && a.accumulate ? was[e] + v[e >> 2][e & 3] : v[e >> 2][e & 3];
+            if (valid) vhap_store8(a.dx, m * a.w.K + k, DT, valid, o);
+        }
     }
 }
 
-// dx[m, k] (+)= sum over the splits: SG threads an element, each every SG-th split, joined in order
+// dx[m, k] (+)= sum over the splits: SG threads an element, each every SG-th split, joined in order.  A block's EL elements are a part of one row's 128.
 template <int DT, int EL, int SG>
-__global__ __launch_bounds__(EL * SG) void mx_join_kernel(const float* __restrict__ part, int splits, long long M, int K, int Kp, void* __restrict__ dx, int accumulate) {
+__global__ __launch_bounds__(EL * SG) void mx_join_kernel(const MxInputGrad a, unsigned blocks) {
     __shared__ float red[SG][EL];
     const int e = threadIdx.x % EL, sg = threadIdx.x / EL;
-    for (long long i0 = (long long)blockIdx.x * EL; i0 < M * K; i0 += (long long)gridDim.x * EL) {
-        const long long i = i0 + e, m = i / K;
-        const int k = (int)(i - m * K);
+    constexpr unsigned BPT = 128 / EL;
+    const size_t Kp = 128 * (size_t)a.ktiles, step = (size_t)a.M * Kp;
+    for (unsigned b = blockIdx.x; b < blocks; b += gridDim.x) {
+        const unsigned tile = b / BPT, m = tile / (unsigned)a.ktiles;
+        const int k = (int)(tile - m * a.ktiles) * 128 + (int)(b % BPT) * EL + e;
+        const float* p = a.part + m * Kp + k;
         float v = 0.f;
-        if (m < M) {
-            const float* p = part + m * Kp + k;
 #pragma unroll 8
-            for (int s = sg; s < splits; s += SG) v += p[(size_t)s * M * Kp];
-        }
+        for (int s = sg; s < (int)a.splits; s += SG) v += p[s * step];
         red[sg][e] = v;
         __syncthreads();
-        if (sg == 0 && m < M) {
+        if (sg == 0 && k < a.w.K) {
 #pragma unroll 8
             for (int j = 1; j < SG; j++) v += red[j][e];
-            if (DT == VHAP_DTYPE_F32 && accumulate) v = static_cast<float*>(dx)[i] + v;
-            mx_put<DT>(dx, i, v);
+            const long long at = (long long)m * a.w.K + k;
+            if (DT == VHAP_DTYPE_F32 && a.accumulate) v = static_cast<float*>(a.dx)[at] + v;
+            mx_put<DT>(a.dx, at, v);
         }
         __syncthreads();
     }
@@ -913,16 +933,16 @@ struct GradPlan {
     long long mtiles, splits, steps_per_wave;
 };
 // how the input's gradient is split: about 1024 blocks in all, each wave at least four steps of 32 rows where there are that many
-GradPlan mx_grad_plan(long long M, long long N, int K) {
+GradPlan mx_grad_plan(long long M, long long N, int K, int dt) {
     GradPlan p;
     p.few = M <= 2;
     p.ktiles = (K + 127) / 128;
-    p.ct = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    p.ct = M <= 16 ? 1 : M <= 32 || dt != VHAP_DTYPE_BF16 ? 2 : 4;                 // (64 rows in several pieces do not fit the registers)
     p.mtiles = p.few ? 1 : (M + 16 * p.ct - 1) / (16 * p.ct);
-    const long long steps = (N + 31) / 32, want = std::max<long long>(1, 1024 / (p.ktiles * p.mtiles));
+    const long long steps = (N + 31) / 32, want = std::max<long long>(1, (p.few ? 512 : 256) / (p.ktiles * p.mtiles)), waves = MX_T / 64;
     p.splits = std::max<long long>(1, std::min(want, (steps + 15) / 16));
-    p.steps_per_wave = (steps + p.splits * 4 - 1) / (p.splits * 4);
-    p.splits = (steps + p.steps_per_wave * 4 - 1) / (p.steps_per_wave * 4);        // (no block without work)
+    p.steps_per_wave = (steps + p.splits * waves - 1) / (p.splits * waves);
+    p.splits = (steps + p.steps_per_wave * waves - 1) / (p.steps_per_wave * waves);  // (no block without work)
     return p;
 }
 
@@ -968,19 +988,20 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
 }
 
 template <int DT>
-int mx_input_grad_launch(const MxInputGrad& a, const GradPlan& p, void* dx, int accumulate, hipStream_t st) {
+int mx_input_grad_launch(const MxInputGrad& a, const GradPlan& p, hipStream_t st) {
     const unsigned grid = (unsigned)(p.splits * p.ktiles * p.mtiles);
     if (p.few) {
         if (a.M == 1) mx_input_grad_few_kernel<DT, 1><<<grid, MX_T, 0, st>>>(a);
         else mx_input_grad_few_kernel<DT, 2><<<grid, MX_T, 0, st>>>(a);
     } else if (p.ct == 1) mx_input_grad_kernel<DT, 1><<<grid, MX_T, 0, st>>>(a);
     else if (p.ct == 2) mx_input_grad_kernel<DT, 2><<<grid, MX_T, 0, st>>>(a);
-    else mx_input_grad_kernel<DT, 4><<<grid, MX_T, 0, st>>>(a);
+    else if constexpr (DT == VHAP_DTYPE_BF16) mx_input_grad_kernel<DT, 4><<<grid, MX_T, 0, st>>>(a);
     VHAP_LAUNCH_CHECK();
-    const long long n = a.M * a.w.K;
+    if (!p.few && p.splits == 1) return VHAP_OK;
+    const unsigned tiles = (unsigned)(a.M * p.ktiles);            // (at most 2^30: the kernel above has a block for every 64 of them; few where there are many splits)
     // many splits of few elements: 64 threads an element; else four
-    if (p.splits > 64) mx_join_kernel<DT, 16, 64><<<(int)std::min((n + 15) / 16, 1ll << 20), 1024, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
-    else mx_join_kernel<DT, 64, 4><<<(int)std::min((n + 63) / 64, 1ll << 20), 256, 0, st>>>(a.part, (int)p.splits, a.M, a.w.K, 128 * p.ktiles, dx, accumulate);
+    if (p.splits > 64) mx_join_kernel<DT, 16, 64><<<std::min(8 * tiles, 1u << 20), 1024, 0, st>>>(a, 8 * tiles);
+    else mx_join_kernel<DT, 64, 4><<<std::min(2 * tiles, 1u << 20), 256, 0, st>>>(a, 2 * tiles);
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
 }
@@ -1027,7 +1048,7 @@ extern "C" int vhap_mx4_linear(const void* x, int dtype, long long ldx, long lon
 
 extern "C" size_t vhap_mx4_linear_input_grad_workspace_bytes(long long M, long long N, int K) {
     if (!mx_dims(N, K) || !mx_dims(M, K) || M == 0 || N == 0) return 0;
-    const GradPlan p = mx_grad_plan(M, N, K);
+    const GradPlan p = mx_grad_plan(M, N, K, VHAP_DTYPE_BF16);                       // (the other types' tiles are no more, and so are their splits)
     return sizeof(float) * (size_t)p.splits * (size_t)M * 128 * (size_t)p.ktiles;
 }
 
@@ -1039,12 +1060,12 @@ extern "C" int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ld
     if (accumulate && dtype != VHAP_DTYPE_F32) return VHAP_E_UNSUPPORTED;
     if (M == 0) return VHAP_OK;
     if (!g || !codes || !scales || !dx || !workspace) return VHAP_E_NULLPTR;
-    const GradPlan p = mx_grad_plan(M, N, K);
+    const GradPlan p = mx_grad_plan(M, N, K, dtype);
     if (p.splits * p.ktiles > MX_MOST_BLOCKS / p.mtiles) return VHAP_E_BADDIM;
     if (workspace_bytes < vhap_mx4_linear_input_grad_workspace_bytes(M, N, K)) return VHAP_E_WORKSPACE;
-    const MxInputGrad a{g, ldg, M, {codes, scales, N, K, mx_kb(K)}, static_cast<float*>(workspace), p.ktiles, (unsigned)p.splits, p.steps_per_wave};
+    const MxInputGrad a{g, ldg, M, {codes, scales, N, K, mx_kb(K)}, static_cast<float*>(workspace), dx, accumulate, p.ktiles, (unsigned)p.splits, p.steps_per_wave};
     int rc = VHAP_OK;
-    MX_BY_TYPE(dtype, rc = mx_input_grad_launch<DT>(a, p, dx, accumulate, vhap_stream(stream)));
+    MX_BY_TYPE(dtype, rc = mx_input_grad_launch<DT>(a, p, vhap_stream(stream)));
     return rc;
 }
 
