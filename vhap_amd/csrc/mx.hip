@@ -609,7 +609,7 @@ template <int DT, int CT>
 __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a) {
     constexpr int P = mx_pieces<DT>(), WAVES = MX_T / 64;
     __shared__ f32x4 red[CT > 1 ? 2 : 1][WAVES][4][2][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
     const int kt = a.kt();
     const unsigned split = a.split();
     const long long m0 = (long long)a.mt() * 16 * CT;
@@ -623,12 +623,18 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a
     const long long n1 = min(n0 + a.steps_per_wave * 32, a.w.rows);
     unsigned nc[8], ns[8];                                        // the next 32 rows, on their way while these are multiplied
     MxRaw8<DT> ng[CT];
+    const unsigned at0 = (unsigned)min(blk, a.w.Kb - 1);
     auto fetch = [&](long long n) {
+        // (the first row's place is the same for the wave; from there 24 bits are enough: a 64-bit product a row and lane cost as much as the matrix instructions)
+        const long long first = min(n, a.w.rows - 1);
+        const int last = (int)min(31ll, a.w.rows - 1 - first);
+        const unsigned* fc = reinterpret_cast<const unsigned*>(a.w.codes) + (size_t)first * a.w.Kb * 4;
+        const uint8_t* fs = a.w.scales + (size_t)first * a.w.Kb;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const size_t at = (size_t)min(n + 8 * q + i, a.w.rows - 1) * a.w.Kb + min(blk, a.w.Kb - 1);
-            nc[i] = reinterpret_cast<const unsigned*>(a.w.codes)[at * 4 + (col & 3)];
-            ns[i] = a.w.scales[at];
+            const unsigned at = __umul24(min(8 * q + i, last), a.w.Kb) + at0;
+            nc[i] = fc[at * 4 + (col & 3)];
+            ns[i] = fs[at];
         }
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
