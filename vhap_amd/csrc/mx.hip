@@ -488,7 +488,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
             mx_settle8<DT>(a.x, min(m0 + 16 * ct + xr, a.M - 1) * a.ldx, 128 * ks + xk, a.w.K, xv[ct]);
             mx_fragments<DT>(xv[ct], f);
 #pragma unroll
-            for (int p = 0; p < P; p++) xs[ct][(tid & 15) & 3][p][((tid & 15) >> 2) * 16 + xr] = f[p];
+            for (int p = 0; p < P; p++) xs[ct][tid & 3][p][((tid & 15) >> 2) * 16 + (xr ^ (tid & 3) << 2)] = f[p];   // (16 neighbouring lanes: 16 places modulo 256 bytes)
         }
         bf16x8 w[NT][4];
 #pragma unroll
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
             for (int ct = 0; ct < CT; ct++)
 #pragma unroll
                 for (int p = P - 1; p >= 0; p--) {                           // (small pieces first)
-                    const bf16x8 b = xs[ct][j][p][lane];
+                    const bf16x8 b = xs[ct][j][p][lane ^ j << 2];
 #pragma unroll
                     for (int t = 0; t < NT; t++) acc[t][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[t][j], b, acc[t][ct], 0, 0, 0);
                 }
