@@ -190,6 +190,7 @@ def test_quantize_shapes_and_strides():
 
 # ---- linear ----
 LINEAR = [(1, 1, 1), (1, 5, 33), (1, 1000, 100), (5, 65, 128), (6, 64, 129), (8, 130, 300), (16, 257, 512), (17, 63, 31), (16, 500, 513), (33, 129, 100), (65, 300, 400),
+          (1, 500, 1024), (16, 70, 1500), (5, 33, 2049), (3, 4100, 1025), (300, 4000, 130), (17, 100001, 33), (6, 100003, 20),
           (2, 4099, 64), (130, 77, 700), (257, 641, 40), (1, 70001, 100), (3, 20011, 100), (20, 9000, 96)]
 
 

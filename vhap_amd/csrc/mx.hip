@@ -524,6 +524,64 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
     }
 }
 
+// Up to 16 rows of x and a long K (beyond what the kernels above hold of x): a block owns 32 rows of W and its eight waves share K, 128 elements at a time by turns, so that few
+// rows of W still give every CU work and a row is read 512 consecutive bytes at a time.  x goes from memory into the fragments, W as above; no barrier before the
+// waves' sums are joined, in order.
+constexpr int MX_LT = 512, MX_LN = 2;                            // threads; tiles of 16 rows of W
+template <int DT>
+__global__ __launch_bounds__(MX_LT) void mx_linear_long_kernel(const MxLinear a) {
+    constexpr int P = mx_pieces<DT>(), WAVES = MX_LT / 64;
+    __shared__ f32x4 red[WAVES][MX_LN][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
+    const long long n0 = (long long)blockIdx.x * 16 * MX_LN, xrow = min((long long)col, a.M - 1) * a.ldx;      // (columns behind M: the last row's, not stored)
+    f32x4 acc[MX_LN];
+#pragma unroll
+    for (int t = 0; t < MX_LN; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 c[MX_LN];
+    unsigned s[MX_LN];
+    MxRaw8<DT> xv[4];
+    auto fetch = [&](int ks) {
+#pragma unroll
+        for (int t = 0; t < MX_LN; t++) c[t] = mx_block(a.w, n0 + 16 * t + (lane >> 2), 4 * ks + (lane & 3), s[t]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) mx_fetch8<DT>(a.x, xrow, 128 * ks + 32 * q + 8 * j, a.w.K, xv[j]);
+    };
+    const int from = 4 * (4 * col + q);
+    const int steps = (a.w.K + 127) / 128;
+    fetch(min(wave, steps - 1));
+    for (int ks = wave; ks < steps; ks += WAVES) {
+        bf16x8 x[4][P], w[MX_LN][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            mx_settle8<DT>(a.x, xrow, 128 * ks + 32 * q + 8 * j, a.w.K, xv[j]);
+            mx_fragments<DT>(xv[j], x[j]);
+        }
+#pragma unroll
+        for (int t = 0; t < MX_LN; t++) {
+            const float sc = mx_scale((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)s[t]));
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[t][j] = mx_decode8((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c[t][j]), sc);
+        }
+        fetch(min(ks + WAVES, steps - 1));
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--)
+#pragma unroll
+                for (int t = 0; t < MX_LN; t++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[t][j], x[j][p], acc[t], 0, 0, 0);
+    }
+#pragma unroll
+    for (int t = 0; t < MX_LN; t++) red[wave][t][lane] = acc[t];
+    __syncthreads();
+    static_assert(16 * 16 * MX_LN == MX_LT, "a thread stores one result");
+    const int i = threadIdx.x % (16 * MX_LN), m = threadIdx.x / (16 * MX_LN);
+    if (m >= a.M || n0 + i >= a.w.rows) return;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) v += red[w][i >> 4][((i >> 2) & 3) * 16 + m][i & 3];
+    mx_put<DT>(a.y, m * a.w.rows + n0 + i, a.bias ? v + a.bias[n0 + i] : v);
+}
+
 // ---- the input's gradient: the sum runs over the rows of W (long), so it is split over blocks and joined by a second launch in a fixed order ----
 struct MxInputGrad {
     const void* g;            // [M, N], rows ldg apart
@@ -976,18 +1034,27 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
         VHAP_LAUNCH_CHECK();
         return VHAP_OK;
     }
-    const int ct = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-    const long long mtiles = (a.M + 16 * ct - 1) / (16 * ct);
-    // 256 rows of W a block, or 128 where that leaves fewer than two blocks a CU
-    const bool wide = mtiles * ((N + 255) / 256) >= 512;
-    const long long tiles = mtiles * ((N + (wide ? 255 : 127)) / (wide ? 256 : 128));
+    const long long cols = (N + 127) / 128;
+    // few rows, few tiles of W and work for all eight waves.  Measured against the tiles below: 1 x 4096 x 4096 bf16 4.9 us against 13.9, 16 x 4096 x 4096 fp32 13.5 / 27.5,
+    // 16 x 16384 x 4096 fp32 28 / 28.5; beyond: 16 x 65536 x 4096 bf16 49 / 34, 16 x 15429 x 512 fp32 9.5 / 5.7
+    if (a.M <= 16 && a.w.K >= 1024 && cols <= 128) {
+        mx_linear_long_kernel<DT><<<(int)((N + 16 * MX_LN - 1) / (16 * MX_LN)), MX_LT, 0, st>>>(a);
+        VHAP_LAUNCH_CHECK();
+        return VHAP_OK;
+    }
+    // Tiles of 16 or 32 rows of x, 64, 128 or 256 rows of W: the smaller ones while the larger would leave CUs idle (256 x 2048 x 400 bf16: 32 x 128 5.5 us, 16 x 128 4.5;
+    // 12 x 15429 x 512 fp32: 16 x 128 6.5, 16 x 64 5.8), the larger ones for reading x and W less often (256 x 15429 x 400 bf16: 16 x 128 14.7, 32 x 128 12.1, 32 x 256
+    // 11.8; 16384 x 1024 x 1024: 69 / 58 / 49).  64 rows of x were no faster (49 us there) and slower where tiles are few.
+    const bool two = (a.M + 31) / 32 * cols >= 256;
+    const long long mtiles = two ? (a.M + 31) / 32 : (a.M + 15) / 16, narrow = mtiles * cols;
+    const int nt = narrow >= 768 ? 4 : narrow > 128 ? 2 : 1;
+    const long long tiles = mtiles * ((N + 64 * nt - 1) / (64 * nt));
     if (tiles > MX_MOST_BLOCKS) return VHAP_E_BADDIM;
 #define MX_LINEAR(NT, CT) mx_linear_kernel<DT, NT, CT><<<(int)tiles, MX_T, 0, st>>>(a, mtiles)
-    if (wide) {
-        if (ct == 1) MX_LINEAR(4, 1); else if (ct == 2) MX_LINEAR(4, 2); else MX_LINEAR(4, 4);
-    } else {
-        if (ct == 1) MX_LINEAR(2, 1); else if (ct == 2) MX_LINEAR(2, 2); else MX_LINEAR(2, 4);
-    }
+    if (two) { if (nt == 4) MX_LINEAR(4, 2); else MX_LINEAR(2, 2); }
+    else if (nt == 4) MX_LINEAR(4, 1);
+    else if (nt == 2) MX_LINEAR(2, 1);
+    else MX_LINEAR(1, 1);
 #undef MX_LINEAR
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
