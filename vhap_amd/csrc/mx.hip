@@ -25,6 +25,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));      // (HIP's uint4 holds a union: arrays of it end up in scratch memory)
 
 constexpr int MX_T = 256;
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_few_kernel(const MxLinear a) {
 // A block's ROWS x NB tile of results out of LDS (rows of NB + 4 floats), 16 threads and more a row, so that a store instruction writes whole lines: out of the matrix
 // instruction's registers a lane's neighbours belong to other rows, and every 16 bytes were a transaction of their own.
 template <int DT, int T, int ROWS, int NB>
-__device__ __forceinline__ void mx_store_tile(const float* tile, void* y, long long M, long long N, const float* bias, int relu, long long m0, long long m_step, long long n0) {
+__device__ __forceinline__ void mx_store_tile(const float* tile, void* y, long long M, long long N, const float* bias, long long m0, long long n0) {
     constexpr int TPR = NB / 8, RP = T / TPR;
     const int c = threadIdx.x % TPR, r0 = threadIdx.x / TPR;
     const long long n = n0 + c * 8;
@@ -437,15 +438,13 @@ __device__ __forceinline__ void mx_store_tile(const float* tile, void* y, long l
     if (bias) vhap_load8(bias, n, VHAP_DTYPE_F32, valid, b);
 #pragma unroll
     for (int r = r0; r < ROWS; r += RP) {
-        const long long m = m0 + (r & 15) + (r >> 4) * m_step;    // (sixteen consecutive rows at a time)
+        const long long m = m0 + r;
         if (m >= M) continue;
         const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + r * (NB + 4) + c * 8), hi = *reinterpret_cast<const f32x4*>(tile + r * (NB + 4) + c * 8 + 4);
         float o[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
+        for (int e = 0; e < 8; e++)
             if (bias) o[e] += b[e];
-            if (relu) o[e] = o[e] < 0.f ? 0.f : o[e];             // (a NaN stays)
-        }
         vhap_store8(y, m * N + n, DT, valid, o);
     }
 }
@@ -520,7 +519,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
 #pragma unroll
         for (int t = 0; t < NT; t++) *reinterpret_cast<f32x4*>(tile + col * (NB + 4) + wave * 16 * NT + 16 * t + 4 * q) = acc[t][ct];
         __syncthreads();
-        mx_store_tile<DT, MX_T, 16, NB>(tile, a.y, a.M, a.w.rows, a.bias, 0, m0 + 16 * ct, 0, n0);
+        mx_store_tile<DT, MX_T, 16, NB>(tile, a.y, a.M, a.w.rows, a.bias, m0 + 16 * ct, n0);
     }
 }
 
@@ -853,12 +852,41 @@ struct MxTile {
 };
 __device__ __forceinline__ int mx_place(int row, int q) { return q ^ ((row >> 1) & 3); }
 
+// two results in 16 bits each
+template <int DT>
+__device__ __forceinline__ unsigned mx_pair(float lo, float hi) {
+    if constexpr (DT == VHAP_DTYPE_BF16) return vhap_bf16_pair(lo, hi);
+    return (unsigned)__half_as_ushort(__float2half_rn(lo)) | (unsigned)__half_as_ushort(__float2half_rn(hi)) << 16;
+}
+// 16 bytes of results, `valid` elements of them (none: not positive), at element i
+template <int DT>
+__device__ __forceinline__ void mx_store16(void* y, long long i, int valid, const u32x4& v) {
+    if constexpr (DT == VHAP_DTYPE_F32) {
+        typedef u32x4 __attribute__((aligned(4))) at4;
+        unsigned* p = static_cast<unsigned*>(y) + i;
+        if (valid >= 4) *reinterpret_cast<at4*>(p) = v;
+        else
+#pragma unroll
+            for (int k = 0; k < 3; k++)
+                if (k < valid) p[k] = v[k];
+    } else {
+        typedef u32x4 __attribute__((aligned(2))) at2;
+        unsigned short* p = static_cast<unsigned short*>(y) + i;
+        if (valid >= 8) *reinterpret_cast<at2*>(p) = v;
+        else
+#pragma unroll
+            for (int k = 0; k < 7; k++)
+                if (k < valid) p[k] = (unsigned short)(v[k >> 1] >> 16 * (k & 1));
+    }
+}
+
 // WHOLE: K is a multiple of a step.  Otherwise every block behind the last is the last one's, with its codes masked to zero in B (as those behind K are, whatever the matrix
 // holds there) and scale 1, and a row's scales are read byte by byte.  Either way the loop has no branch: a branch around a load made the compiler wait for it there.
 template <int DT, int BM, int BN, bool WHOLE>
 __global__ __launch_bounds__(MX_T) void mx_matmul_kernel(const MxMatmul a, long long mtiles) {
     constexpr int TM = BM / 32, TN = BN / 32, CA = BM / 64, CB = BN / 64;        // tiles a wave; rows a thread carries a block of
-    constexpr size_t OPERANDS = 2 * (sizeof(MxTile<BM>) + sizeof(MxTile<BN>)), RESULTS = sizeof(float) * 32 * (BN + 4);
+    constexpr int SIZE = DT == VHAP_DTYPE_F32 ? 4 : 2;
+    constexpr size_t OPERANDS = 2 * (sizeof(MxTile<BM>) + sizeof(MxTile<BN>)), RESULTS = (SIZE == 4 ? BM / 2 : BM) * (BN * SIZE + 16);
     static_assert(BM + BN <= MX_T, "a thread carries the scales of one row");
     __shared__ __attribute__((aligned(16))) unsigned char lds[OPERANDS > RESULTS ? OPERANDS : RESULTS];
     auto ta = reinterpret_cast<MxTile<BM>*>(lds);
@@ -956,15 +984,40 @@ __global__ __launch_bounds__(MX_T) void mx_matmul_kernel(const MxMatmul a, long 
         __syncthreads();
     }
     multiply(buf);
-    __syncthreads();
-    float* tile = reinterpret_cast<float*>(lds);
+    // the results, biased and rounded, through LDS (whole lines out): all rows at once in 16 bits, a half of each wave's in fp32
+    constexpr int ROUNDS = DT == VHAP_DTYPE_F32 ? 2 : 1, RT = TM / ROUNDS, PITCH = (BN + 16 / SIZE) * SIZE;
+    float b[TN][4];
 #pragma unroll
-    for (int u = 0; u < TM; u++) {
-        if (u) __syncthreads();
+    for (int t = 0; t < TN; t++)
 #pragma unroll
-        for (int t = 0; t < TN; t++) *reinterpret_cast<f32x4*>(tile + ((wave & 1) * 16 + col) * (BN + 4) + wn + 16 * t + 4 * q) = acc[t][u];
+        for (int i = 0; i < 4; i++) b[t][i] = a.bias ? a.bias[min(n0 + wn + 16 * t + 4 * q + i, a.b.rows - 1)] : 0.f;
+#pragma unroll
+    for (int round = 0; round < ROUNDS; round++) {
         __syncthreads();
-        mx_store_tile<DT, MX_T, 32, BN>(tile, a.y, a.a.rows, a.b.rows, a.bias, a.relu, m0 + 16 * u, BM / 2, n0);
+#pragma unroll
+        for (int u = 0; u < RT; u++)
+#pragma unroll
+            for (int t = 0; t < TN; t++) {
+                f32x4 v = acc[t][round * RT + u];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (a.bias) v[i] += b[t][i];
+                    if (a.relu) v[i] = v[i] < 0.f ? 0.f : v[i];   // (a NaN stays)
+                }
+                unsigned char* at = lds + ((wave & 1) * 16 * RT + 16 * u + col) * PITCH + (wn + 16 * t + 4 * q) * SIZE;
+                if constexpr (DT == VHAP_DTYPE_F32) *reinterpret_cast<f32x4*>(at) = v;
+                else *reinterpret_cast<u32x2*>(at) = u32x2{mx_pair<DT>(v[0], v[1]), mx_pair<DT>(v[2], v[3])};
+            }
+        __syncthreads();
+        constexpr int TPR = BN * SIZE / 16, PER = 16 / SIZE;      // threads a row, elements each
+        const int c = tid % TPR;
+        const long long n = n0 + c * PER;
+#pragma unroll
+        for (int r = tid / TPR; r < 32 * RT; r += MX_T / TPR) {
+            const long long m = m0 + (r / (16 * RT)) * (BM / 2) + round * 16 * RT + r % (16 * RT);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * PITCH + c * 16);
+            if (m < a.a.rows) mx_store16<DT>(a.y, m * a.b.rows + n, (int)min((long long)PER, a.b.rows - n), v);
+        }
     }
 }
 
