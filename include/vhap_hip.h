@@ -719,7 +719,7 @@ int vhap_adam_step(int n_tensors, float* const* params, const float* const* grad
  * vhap_adam_step_clipped: vhap_adam_step on round(grads * c), the gradients left as they are, the norm over these n_tensors (2-norm; norm may be NULL):
  *   the counter is advanced by the call's own launches (no third one).  call_flags as vhap_adam_step.  The hyperparameters are 64-bit: 1 - beta and
  *   1 - beta^step are formed there and rounded to float32 once (vhap_adam_step forms them in float32: its 1 - beta2 is off by 1.3e-5 at beta2 = 0.999).
- * Lists of at most 64 units of 2 KB (no unit crosses a tensor) are one launch, others two, and two more for every further 128 tensors that do not lie one
+ * Lists of at most 32 units of 2 KB (no unit crosses a tensor) are one launch, others two, and two more for every further 128 tensors that do not lie one
  * behind another in memory. */
 #define VHAP_NORM_INF 0
 #define VHAP_DTYPE_F32 0

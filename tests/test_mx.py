@@ -484,3 +484,16 @@ def test_a_captured_backward():
         y1 = mx.linear(x1, w, bias.detach())
         assert torch.equal(y.detach(), y1.detach()) and torch.equal(dx, torch.autograd.grad(y1, x1, g)[0])
         assert torch.equal(db, torch.autograd.grad(mx.linear(x1, w, b1 := bias.detach().clone().requires_grad_()), b1, g)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k", [(270001, 100), (2 ** 20 + 37, 7), (81000, 401)])
+def test_one_row_against_a_large_matrix(n, k):
+    w = random_mx(n, k, 1)
+    g, x = randn((1, n), 2), randn((1, k), 3)
+    W, G, X = w.dequantize().double(), g.double(), x.double()                    # (dequantize is tested above)
+    check_sum(mx.linear_input_grad(g, w), (G @ W).cpu(), (G.abs() @ W.abs()).cpu(), n + 1024, torch.float32)
+    check_sum(mx.linear(x, w), (X @ W.t()).cpu(), (X.abs() @ W.abs().t()).cpu(), k, torch.float32)
+    w.scales[n - 1, 0] = 255                                                     # the last row's first block alone
+    dx = mx.linear_input_grad(g, w)
+    assert dx[:, :32].isnan().all() and not dx[:, 32:].isnan().any()

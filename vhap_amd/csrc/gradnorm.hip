@@ -23,7 +23,7 @@ namespace {
 constexpr int GN_T = 1024, GN_WAVES = GN_T / 64, GN_BLOCKS = 256, GN_UNIT = 2048;
 constexpr int GN_MAX = 128;                 // tensors per launch: the table travels as kernel arguments (under 4 KB), so a capture keeps it by value
 constexpr long long GN_MOST = 1ll << 38;    // elements of a list: its units are counted in 32 bits
-constexpr int ONE_BLOCK_UNITS = 64;
+constexpr int ONE_BLOCK_UNITS = 32;         // 16 units in one launch 5.6 us, in two 8.6; 48 8.6 / 8.7; 24 of 24 tensors 11.9 / 11.5, 48 of 48 18.4 / 12.7
 
 template <int MAX>
 struct GnTableOf {

@@ -49,17 +49,6 @@ __device__ __forceinline__ u32x4 mx_block(const MxMatrix& w, long long row, int 
     return reinterpret_cast<const u32x4*>(w.codes)[at];
 }
 
-// The same for a matrix instruction's operand: lane (r, q) = (lane % 16, lane / 16) gets block k + q of row row_of(r).  Read in that order, sixteen neighbouring lanes would
-// touch sixteen rows, four times over; read four lanes a row and passed on across the wave, neighbours read 64 consecutive bytes.
-template <typename F>
-__device__ __forceinline__ u32x4 mx_operand(const MxMatrix& w, F row_of, int k, unsigned& scale) {
-    const int lane = threadIdx.x & 63, from = 4 * (4 * (lane & 15) + (lane >> 4));
-    const u32x4 c = mx_block(w, row_of(lane >> 2), k + (lane & 3), scale);
-    scale = (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)scale);
-    return u32x4{(unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.x), (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.y),
-                 (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.z), (unsigned)__builtin_amdgcn_ds_bpermute(from, (int)c.w)};
-}
-
 __device__ __forceinline__ unsigned mx_pair_bits(bf16x2 v) { return __builtin_bit_cast(unsigned, v); }
 
 // eight codes (one dword) -> eight bf16 numbers
@@ -253,21 +242,6 @@ struct MxLinear {
     void* y;                  // [M, N]
 };
 
-// NT * 4 consecutive columns n of row m
-template <int DT, int NT>
-__device__ __forceinline__ void mx_store_row(const MxLinear& a, long long m, long long n, const float (&v)[NT * 4]) {
-#pragma unroll
-    for (int h = 0; h < NT * 4; h += 8) {
-        const int valid = mx_left(n + h, a.w.rows);
-        if (valid == 0) continue;
-        float o[8], b[8];
-        if (a.bias) vhap_load8(a.bias, n + h, VHAP_DTYPE_F32, valid, b);
-#pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = a.bias ? v[h + e] + b[e] : v[h + e];
-        vhap_store8(a.y, m * a.w.rows + n + h, DT, valid, o);
-    }
-}
-
 template <int DT>
 __device__ __forceinline__ float mx_one(const void* p, long long i) {
     if constexpr (DT == VHAP_DTYPE_F32) return static_cast<const float*>(p)[i];
@@ -364,67 +338,6 @@ __global__ __launch_bounds__(MX_T) void mx_linear_row_kernel(const MxLinear a) {
     }
 }
 
-// Few rows of x (M times its pieces fit the 16 columns of ONE matrix instruction) and K up to 128 KS: the x fragments stay in registers, every wave streams groups of
-// 64 rows of W through them.  Column c holds piece c % P of row c / P; the pieces' sums are joined across neighbouring lanes at the end.
-// Operand rows are dealt out so that a lane ends with 16 CONSECUTIVE columns of y: tile t, row r of the instruction is row 16 (r / 4) + 4 t + r % 4 of the group.
-template <int DT, int KS>
-__global__ __launch_bounds__(MX_T) void mx_linear_few_kernel(const MxLinear a) {
-    constexpr int P = mx_pieces<DT>();
-    const int lane = threadIdx.x & 63, col = lane & 15, q = lane >> 4;
-    const int m = col / P, p = col % P;
-    __shared__ __attribute__((aligned(16))) float xs[16 / P][128 * KS];
-    for (int i = threadIdx.x; i < 16 / P * 128 * KS; i += MX_T) {
-        const int row = i / (128 * KS), k = i % (128 * KS);
-        xs[row][k] = row < a.M && k < a.w.K ? mx_one<DT>(a.x, row * a.ldx + k) : 0.f;
-    }
-    __syncthreads();
-    bf16x8 xb[KS][4];
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float* src = xs[min(m, 16 / P - 1)] + 128 * ks + 32 * q + 8 * j;
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(src), hi = *reinterpret_cast<const f32x4*>(src + 4);
-            const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            bf16x8 f[P];
-            mx_split8<P>(v, f);
-            xb[ks][j] = f[0];
-            if constexpr (P > 1) xb[ks][j] = p == 1 ? f[1] : xb[ks][j];
-            if constexpr (P > 2) xb[ks][j] = p == 2 ? f[2] : xb[ks][j];
-        }
-    const long long groups = (a.w.rows + 63) / 64;
-    for (long long g = (long long)blockIdx.x * (MX_T / 64) + (threadIdx.x >> 6); g < groups; g += (long long)gridDim.x * (MX_T / 64)) {
-        const long long base = g * 64;
-        u32x4 c[4][KS];
-        unsigned s[4][KS];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) c[t][ks] = mx_operand(a.w, [&](int r) { return base + 16 * (r >> 2) + 4 * t + (r & 3); }, 4 * ks, s[t][ks]);
-        float v[16];
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const float sc = mx_scale(s[t][ks]);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode8(c[t][ks].x, sc), xb[ks][0], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode8(c[t][ks].y, sc), xb[ks][1], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode8(c[t][ks].z, sc), xb[ks][2], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode8(c[t][ks].w, sc), xb[ks][3], acc, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float r = acc[i];
-                if constexpr (P > 1) r += vhap_dpp<0x101>(acc[i]);          // row_shl 1: the next lane's
-                if constexpr (P > 2) r += vhap_dpp<0x102>(acc[i]);
-                v[4 * t + i] = r;
-            }
-        }
-        if (p == 0 && m < a.M && m < 16 / P) mx_store_row<DT, 4>(a, m, base + 16 * q, v);
-    }
-}
-
 // A block's ROWS x NB tile of results out of LDS (rows of NB + 4 floats), 16 threads and more a row, so that a store instruction writes whole lines: out of the matrix
 // instruction's registers a lane's neighbours belong to other rows, and every 16 bytes were a transaction of their own.
 template <int DT, int T, int ROWS, int NB>
@@ -478,7 +391,9 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
             mx_fetch8<DT>(a.x, min(m0 + 16 * ct + xr, a.M - 1) * a.ldx, 128 * ks + xk, a.w.K, xv[ct]);
         }
     };
-    const int from = 4 * (4 * col + q);                                      // (mx_operand, with the loads ahead of their use)
+    // the instruction wants block 4 ks + q of row `col` in lane (col, q); read in that order, sixteen neighbouring lanes would touch sixteen rows, four times over: read four
+    // lanes a row and passed on across the wave, neighbours read 64 consecutive bytes
+    const int from = 4 * (4 * col + q);
     fetch(0);
     for (int ks = 0; ks * 128 < a.w.K; ks++) {
 #pragma unroll
@@ -586,7 +501,7 @@ struct MxInputGrad {
     const void* g;            // [M, N], rows ldg apart
     long long ldg, M;
     MxMatrix w;               // [N, K]
-    float* part;              // [splits, M, 128 ktiles], for more than one split or one or two rows
+    float* part;              // [splits, M, 128 ktiles], for more than one split or mx_input_grad_row_kernel
     void* dx;
     int accumulate;
     int ktiles;
@@ -598,65 +513,51 @@ struct MxInputGrad {
     __device__ __forceinline__ unsigned mt() const { return blockIdx.x / splits / (unsigned)ktiles; }
 };
 
-// One or two rows of g: per 16 rows of W a lane decodes one block of 32 (four lanes a row) and adds it, times g, to its 32 sums -- 16 conversions and 32 M
+// One row of g, fp32: per 16 rows of W a lane decodes one block of 32 (four lanes a row) and adds it, times g, to its 32 sums -- 16 conversions and 32 M
 // multiply-adds for 16 bytes, under what memory delivers.
-template <int DT, int MM>
-__global__ __launch_bounds__(MX_T) void mx_input_grad_few_kernel(const MxInputGrad a) {
-    __shared__ float red[MX_T / 64][MM][128];
+__global__ __launch_bounds__(MX_T) void mx_input_grad_row_kernel(const MxInputGrad a) {
+    __shared__ float red[MX_T / 64][32][64 + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = lane & 3, r = lane >> 2;
     const int kt = a.kt(), blk = 4 * kt + b;
     const unsigned split = a.split();
-    float acc[MM][32];
+    const float* const gp = static_cast<const float*>(a.g);
+    float acc[32];
 #pragma unroll
-    for (int m = 0; m < MM; m++)
-#pragma unroll
-        for (int e = 0; e < 32; e++) acc[m][e] = 0.f;
+    for (int e = 0; e < 32; e++) acc[e] = 0.f;
     const long long n0 = ((long long)split * (MX_T / 64) + wave) * a.steps_per_wave * 32;
     const long long n1 = min(n0 + a.steps_per_wave * 32, a.w.rows);
     for (long long n = n0; n < n1; n += 32) {
         u32x4 c[2];
         unsigned s[2];
-        float g[2][MM];
+        float g[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const long long row = n + 16 * u + r;
             c[u] = mx_block(a.w, row, blk, s[u]);
-#pragma unroll
-            for (int m = 0; m < MM; m++) {
-                g[u][m] = 0.f;
-                if (row < a.w.rows && m < a.M) {
-                    const long long at = m * a.ldg + row;
-                    g[u][m] = mx_one<DT>(a.g, at);
-                }
-            }
+            g[u] = row < a.w.rows ? gp[row] : 0.f;
         }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             float w[32];
             mx_decode32(c[u], mx_scale(s[u]), w);
 #pragma unroll
-            for (int m = 0; m < MM; m++)
-#pragma unroll
-                for (int e = 0; e < 32; e++) acc[m][e] = fmaf(w[e], g[u][m], acc[m][e]);
+            for (int e = 0; e < 32; e++) acc[e] = fmaf(w[e], g[u], acc[e]);
         }
     }
-    // the 16 lanes that share a block, then the four waves
+    // the 16 lanes of four waves that share a block, in order: a thread two waves' of one element
 #pragma unroll
-    for (int m = 0; m < MM; m++)
-#pragma unroll
-        for (int e = 0; e < 32; e++) {
-            float v = acc[m][e];
-            v += vhap_dpp<0x124>(v);                             // row_ror 4
-            v += vhap_dpp<0x128>(v);                             // row_ror 8
-            v += __shfl_xor(v, 16, 64);
-            v += __shfl_xor(v, 32, 64);
-            if (r == 0) red[wave][m][32 * b + e] = v;
-        }
+    for (int e = 0; e < 32; e++) red[wave][e][lane] = acc[e];
     __syncthreads();
-    for (int i = threadIdx.x; i < MM * 128; i += MX_T) {
-        const int m = i >> 7, k = i & 127;
-        if (m < a.M) a.part[((size_t)split * a.M + m) * (128 * a.ktiles) + 128 * kt + k] = (red[0][m][k] + red[1][m][k]) + (red[2][m][k] + red[3][m][k]);
-    }
+    const int k = threadIdx.x & 127, half = threadIdx.x >> 7;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) v += red[2 * half + w][k & 31][4 * i + (k >> 5)];
+    __syncthreads();
+    if (half) red[k >> 6][0][k & 63] = v;
+    __syncthreads();
+    if (!half) a.part[(size_t)split * (128 * a.ktiles) + 128 * kt + k] = v + red[k >> 6][0][k & 63];
 }
 
 // Any number of rows of g.  The sum runs along W's rows while its codes lie along K: a lane takes eight rows x eight elements of K (eight dwords), decodes them and turns
@@ -799,7 +700,7 @@ __global__ __launch_bounds__(EL * SG) void mx_join_kernel(const MxInputGrad a, u
 template <int DT, int RG>
 __global__ __launch_bounds__(MX_T) void mx_colsum_kernel(const void* __restrict__ g, long long ldg, long long M, long long N, float* __restrict__ out) {
     constexpr int CG = MX_T / RG;
-    __shared__ float red[RG > 1 ? RG : 1][RG > 1 ? CG : 1][8 + 1];
+    __shared__ float red[RG][CG][8 + 1];
     const int c = threadIdx.x % CG, r = threadIdx.x / CG;
     const long long n = ((long long)blockIdx.x * CG + c) * 8;
     const int valid = mx_left(n, N);
@@ -822,16 +723,16 @@ __global__ __launch_bounds__(MX_T) void mx_colsum_kernel(const void* __restrict_
             for (int e = 0; e < 8; e++) v[e] += x[e];
         }
     }
-    if constexpr (RG > 1) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) red[r][c][e] = v[e];
-        __syncthreads();
-        if (r > 0) return;
-        for (int j = 1; j < RG; j++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] += red[j][c][e];
-    }
-    if (valid) vhap_store8(out, n, VHAP_DTYPE_F32, valid, v);
+    for (int e = 0; e < 8; e++) red[r][c][e] = v[e];
+    __syncthreads();
+    const int own = threadIdx.x;                                 // a thread joins one column
+    const long long at = (long long)blockIdx.x * CG * 8 + own;
+    if (own >= CG * 8 || at >= N) return;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int j = 0; j < RG; j++) sum += red[j][own >> 3][own & 7];
+    out[at] = sum;
 }
 
 // ---- matmul: both operands in 4 bits ----
@@ -1048,17 +949,19 @@ inline int mx_grid(long long items, int most) { return (int)std::min<long long>(
 
 struct GradPlan {
     int ktiles, ct;
-    bool few;
+    bool row;
     long long mtiles, splits, steps_per_wave;
 };
 // how the input's gradient is split: about 1024 blocks in all, each wave at least four steps of 32 rows where there are that many
 GradPlan mx_grad_plan(long long M, long long N, int K, int dt) {
     GradPlan p;
-    p.few = M <= 2;
+    // one fp32 row against a large W is the vector unit's work (1 x 786432 x 100: ROWA us, by the matrix instruction ROWB), anything else the matrix instruction's (1 x 200000 x 100:
+    // 12 us both; 1 x 15429 x 400 fp32 10 / 9, bf16 11 / 8)
+    p.row = M == 1 && dt == VHAP_DTYPE_F32 && N * mx_kb(K) >= (1 << 20);
     p.ktiles = (K + 127) / 128;
     p.ct = M <= 16 ? 1 : M <= 32 || dt != VHAP_DTYPE_BF16 ? 2 : 4;                 // (64 rows in several pieces do not fit the registers)
-    p.mtiles = p.few ? 1 : (M + 16 * p.ct - 1) / (16 * p.ct);
-    const long long steps = (N + 31) / 32, want = std::max<long long>(1, (p.few ? 512 : 256) / (p.ktiles * p.mtiles)), waves = MX_T / 64;
+    p.mtiles = p.row ? 1 : (M + 16 * p.ct - 1) / (16 * p.ct);
+    const long long steps = (N + 31) / 32, want = std::max<long long>(1, (p.row ? 512 : 256) / (p.ktiles * p.mtiles)), waves = MX_T / 64;
     p.splits = std::max<long long>(1, std::min(want, (steps + 15) / 16));
     p.steps_per_wave = (steps + p.splits * waves - 1) / (p.splits * waves);
     p.splits = (steps + p.steps_per_wave * waves - 1) / (p.steps_per_wave * waves);  // (no block without work)
@@ -1067,7 +970,6 @@ GradPlan mx_grad_plan(long long M, long long N, int K, int dt) {
 
 template <int DT>
 int mx_linear_launch(const MxLinear& a, hipStream_t st) {
-    constexpr int P = mx_pieces<DT>();
     const long long N = a.w.rows;
     const int ks = (a.w.K + 127) / 128;
     if (a.M <= 2 && ks <= (a.M == 1 ? 4 : 2)) {
@@ -1078,14 +980,6 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
         } else if (ks == 1) mx_linear_row_kernel<DT, 1, 1><<<grid, MX_T, 0, st>>>(a);
         else if (ks == 2) mx_linear_row_kernel<DT, 1, 2><<<grid, MX_T, 0, st>>>(a);
         else mx_linear_row_kernel<DT, 1, 4><<<grid, MX_T, 0, st>>>(a);
-        VHAP_LAUNCH_CHECK();
-        return VHAP_OK;
-    }
-    if (a.M * P <= 16 && ks <= 4) {
-        const int grid = mx_grid((N + 63) / 64 * 64, 2048);
-        if (ks == 1) mx_linear_few_kernel<DT, 1><<<grid, MX_T, 0, st>>>(a);
-        else if (ks == 2) mx_linear_few_kernel<DT, 2><<<grid, MX_T, 0, st>>>(a);
-        else mx_linear_few_kernel<DT, 4><<<grid, MX_T, 0, st>>>(a);
         VHAP_LAUNCH_CHECK();
         return VHAP_OK;
     }
@@ -1118,14 +1012,13 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
 template <int DT>
 int mx_input_grad_launch(const MxInputGrad& a, const GradPlan& p, hipStream_t st) {
     const unsigned grid = (unsigned)(p.splits * p.ktiles * p.mtiles);
-    if (p.few) {
-        if (a.M == 1) mx_input_grad_few_kernel<DT, 1><<<grid, MX_T, 0, st>>>(a);
-        else mx_input_grad_few_kernel<DT, 2><<<grid, MX_T, 0, st>>>(a);
+    if (p.row) {
+        mx_input_grad_row_kernel<<<grid, MX_T, 0, st>>>(a);
     } else if (p.ct == 1) mx_input_grad_kernel<DT, 1><<<grid, MX_T, 0, st>>>(a);
     else if (p.ct == 2) mx_input_grad_kernel<DT, 2><<<grid, MX_T, 0, st>>>(a);
     else if constexpr (DT == VHAP_DTYPE_BF16) mx_input_grad_kernel<DT, 4><<<grid, MX_T, 0, st>>>(a);
     VHAP_LAUNCH_CHECK();
-    if (!p.few && p.splits == 1) return VHAP_OK;
+    if (!p.row && p.splits == 1) return VHAP_OK;
     const unsigned tiles = (unsigned)(a.M * p.ktiles);            // (at most 2^30: the kernel above has a block for every 64 of them; few where there are many splits)
     // many splits of few elements: 64 threads an element; else four
     if (p.splits > 64) mx_join_kernel<DT, 16, 64><<<std::min(8 * tiles, 1u << 20), 1024, 0, st>>>(a, 8 * tiles);
@@ -1176,8 +1069,9 @@ extern "C" int vhap_mx4_linear(const void* x, int dtype, long long ldx, long lon
 
 extern "C" size_t vhap_mx4_linear_input_grad_workspace_bytes(long long M, long long N, int K) {
     if (!mx_dims(N, K) || !mx_dims(M, K) || M == 0 || N == 0) return 0;
-    const GradPlan p = mx_grad_plan(M, N, K, VHAP_DTYPE_BF16);                       // (the other types' tiles are no more, and so are their splits)
-    return sizeof(float) * (size_t)p.splits * (size_t)M * 128 * (size_t)p.ktiles;
+    // (the types differ in their splits: bf16 has the largest tiles and so the most splits, except where an fp32 row goes its own way)
+    const GradPlan p = mx_grad_plan(M, N, K, VHAP_DTYPE_BF16), row = mx_grad_plan(M, N, K, VHAP_DTYPE_F32);
+    return sizeof(float) * (size_t)std::max(p.splits, row.splits) * (size_t)M * 128 * (size_t)p.ktiles;
 }
 
 extern "C" int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ldg, long long M, const uint8_t* codes, const uint8_t* scales, long long N, int K,
@@ -1199,12 +1093,13 @@ extern "C" int vhap_mx4_linear_input_grad(const void* g, int dtype, long long ld
 
 extern "C" int vhap_mx4_column_sums(const void* g, int dtype, long long ldg, long long M, long long N, float* out, vhap_stream_t stream) {
     VHAP_ENTER();
-    if (!mx_dims(M, 1) || !mx_dims(N, 1) || !mx_dt(dtype) || ldg < 0 || N / (8 * MX_T) >= MX_MOST_BLOCKS) return VHAP_E_BADDIM;
+    if (!mx_dims(M, 1) || !mx_dims(N, 1) || !mx_dt(dtype) || ldg < 0 || N / MX_T >= MX_MOST_BLOCKS) return VHAP_E_BADDIM;
     if (N == 0) return VHAP_OK;
     if (!out || (M > 0 && !g)) return VHAP_E_NULLPTR;
-    // few rows: every thread sums its own columns; from eight rows on 64 threads share them (32 columns a block, as long as a grid has room for that)
-    if (M < 8 || N / 32 >= MX_MOST_BLOCKS) MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 1><<<vhap_cdiv(N, 8 * MX_T), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)))
-    else MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 64><<<vhap_cdiv(N, 8 * MX_T / 64), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)));
+    // 64 runs of rows where there are many rows and few columns, else 8 (256 x 15429 bf16: 7 us with 64, 21 with 8; 256 x 786432: 128 / 74; 8 x 15429: 2.7 / 2.5;
+    // every thread by itself: 116, 142, 5.5)
+    if (M >= 32 && N <= 65536) MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 64><<<vhap_cdiv(N, 8 * MX_T / 64), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)))
+    else MX_BY_TYPE(dtype, (mx_colsum_kernel<DT, 8><<<vhap_cdiv(N, 8 * MX_T / 8), MX_T, 0, vhap_stream(stream)>>>(g, ldg, M, N, out)));
     VHAP_LAUNCH_CHECK();
     return VHAP_OK;
 }
@@ -1217,8 +1112,9 @@ extern "C" int vhap_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, 
     if (!a_codes || !a_scales || !b_codes || !b_scales || !y) return VHAP_E_NULLPTR;
     const int Kb = mx_kb(K);
     const MxMatmul a{{a_codes, a_scales, M, K, Kb}, {b_codes, b_scales, N, K, Kb}, bias, (call_flags & VHAP_CONV_OUT_RELU) ? 1 : 0, y};
-    // large tiles where they fill the chip, small ones where they would leave it empty
-    const bool large = ((M + 127) / 128) * ((N + 127) / 128) >= 256;
+    // large tiles where they fill the chip, small ones where they would leave CUs idle (4096 x 1024 x 1024 to bf16, 256 large tiles: 10.4 us, with small ones 8.5;
+    // 6144 x 1024 x 1024, 384: 12.8 / 14.5; 16384 x 1024 x 1024: 22.7 / 31.7)
+    const bool large = ((M + 127) / 128) * ((N + 127) / 128) >= 384;
     int rc = VHAP_OK;
     MX_BY_TYPE(dtype, (rc = large ? mx_matmul_launch<DT, 128, 128>(a, vhap_stream(stream)) : mx_matmul_launch<DT, 64, 64>(a, vhap_stream(stream))));
     return rc;
