@@ -180,7 +180,7 @@ __device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[
 __device__ __forceinline__ int mx_left(long long at, long long end) { return at >= end ? 0 : end - at < 8 ? (int)(end - at) : 8; }
 
 // ---- quantise / dequantise: four lanes a block, eight elements a lane (16 or 32 contiguous bytes of x, one dword of codes) ----
-// Index: unsigned where rows x blocks x 4 is below 2^31 (a 64-bit division is a hundred instructions), long long beyond.
+// Index: unsigned where rows x blocks x 4 is below 2^31, long long beyond (a 64-bit division is a hundred instructions: 1000 x 1000 bf16 there and back 4.6 us / 4.9).
 template <int DT, typename Index>
 __global__ __launch_bounds__(MX_T) void mx_quantize_kernel(const void* __restrict__ x, long long ldx, long long rows, int K, int Kb, uint8_t* __restrict__ codes,
                                                            uint8_t* __restrict__ scales) {
@@ -952,16 +952,18 @@ struct GradPlan {
     bool row;
     long long mtiles, splits, steps_per_wave;
 };
-// how the input's gradient is split: about 1024 blocks in all, each wave at least four steps of 32 rows where there are that many
+// how the input's gradient is split: about 256 blocks in all, each wave at least four steps of 32 rows where there are that many (512 and 1024 blocks write and read more partial sums:
+// 256 x 15429 x 400 fp32 34 us with 256, 47 with 512 and 1024; 64 x 786432 x 100 bf16 48 / 52 / 66), 1024 where a row goes its own way (1 x 200000 x 400 15 us, 26 with 512;
+// 1 x 786432 x 100 15.6 / 14.8)
 GradPlan mx_grad_plan(long long M, long long N, int K, int dt) {
     GradPlan p;
-    // one fp32 row against a large W is the vector unit's work (1 x 786432 x 100: ROWA us, by the matrix instruction ROWB), anything else the matrix instruction's (1 x 200000 x 100:
-    // 12 us both; 1 x 15429 x 400 fp32 10 / 9, bf16 11 / 8)
+    // one fp32 row against a large W is the vector unit's work (1 x 786432 x 100: 15.6 us, by the matrix instruction 26; 1 x 200000 x 400 15 / 27), anything else the matrix instruction's
+    // (1 x 200000 x 100: 12 us both; 1 x 15429 x 400 fp32 10 / 9, bf16 11 / 8)
     p.row = M == 1 && dt == VHAP_DTYPE_F32 && N * mx_kb(K) >= (1 << 20);
     p.ktiles = (K + 127) / 128;
     p.ct = M <= 16 ? 1 : M <= 32 || dt != VHAP_DTYPE_BF16 ? 2 : 4;                 // (64 rows in several pieces do not fit the registers)
     p.mtiles = p.row ? 1 : (M + 16 * p.ct - 1) / (16 * p.ct);
-    const long long steps = (N + 31) / 32, want = std::max<long long>(1, (p.row ? 512 : 256) / (p.ktiles * p.mtiles)), waves = MX_T / 64;
+    const long long steps = (N + 31) / 32, want = std::max<long long>(1, (p.row ? 1024 : 256) / (p.ktiles * p.mtiles)), waves = MX_T / 64;
     p.splits = std::max<long long>(1, std::min(want, (steps + 15) / 16));
     p.steps_per_wave = (steps + p.splits * waves - 1) / (p.splits * waves);
     p.splits = (steps + p.steps_per_wave * waves - 1) / (p.steps_per_wave * waves);  // (no block without work)
@@ -972,7 +974,9 @@ template <int DT>
 int mx_linear_launch(const MxLinear& a, hipStream_t st) {
     const long long N = a.w.rows;
     const int ks = (a.w.K + 127) / 128;
-    if (a.M <= 2 && ks <= (a.M == 1 ? 4 : 2)) {
+    // one or two rows: against the tiles below 1 x 786432 x 100 fp32 11.6 us / 28, 2 x 786432 x 100 13.6 / 27, 1 x 1000 x 100 2.7 / 3.3; a longer K only pays for many rows of W
+    // (1 x 200000 x 500 fp32 14.5 / 30, 1 x 50000 x 400 bf16 4.9 / 6.6, 1 x 15429 x 400 4.7 / 4.1); four rows by this way were 4.2 us / 3.5 against 15429 x 100
+    if (a.M <= 2 && (ks == 1 || (N >= 32768 && ks <= (a.M == 1 ? 4 : 2)))) {
         const int grid = mx_grid((N + 63) / 64 * 64, 1024);
         if (a.M == 2) {
             if (ks == 1) mx_linear_row_kernel<DT, 2, 1><<<grid, MX_T, 0, st>>>(a);
@@ -1020,7 +1024,7 @@ int mx_input_grad_launch(const MxInputGrad& a, const GradPlan& p, hipStream_t st
     VHAP_LAUNCH_CHECK();
     if (!p.row && p.splits == 1) return VHAP_OK;
     const unsigned tiles = (unsigned)(a.M * p.ktiles);            // (at most 2^30: the kernel above has a block for every 64 of them; few where there are many splits)
-    // many splits of few elements: 64 threads an element; else four
+    // many splits of few elements: 64 threads an element, else four (1 x 786432 x 100: 17.7 us, 22 with four; 256 x 15429 x 400 24, 48 with 64)
     if (p.splits > 64) mx_join_kernel<DT, 16, 64><<<std::min(8 * tiles, 1u << 20), 1024, 0, st>>>(a, 8 * tiles);
     else mx_join_kernel<DT, 64, 4><<<std::min(2 * tiles, 1u << 20), 256, 0, st>>>(a, 2 * tiles);
     VHAP_LAUNCH_CHECK();
