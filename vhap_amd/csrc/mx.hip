@@ -180,6 +180,7 @@ __device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[
 __device__ __forceinline__ int mx_left(long long at, long long end) { return at >= end ? 0 : end - at < 8 ? (int)(end - at) : 8; }
 
 // ---- quantise / dequantise: four lanes a block, eight elements a lane (16 or 32 contiguous bytes of x, one dword of codes) ----
+// Bound by HBM: 786432 x 100 fp32 -> codes 64 us (356 MB, 5.6 TB/s), codes -> bf16 40 us (199 MB, 5.0 TB/s); small ones by the launch (1023 x 257: 2.5 us each).
 // Index: unsigned where rows x blocks x 4 is below 2^31, long long beyond (a 64-bit division is a hundred instructions: 1000 x 1000 bf16 there and back 4.6 us / 4.9).
 template <int DT, typename Index>
 __global__ __launch_bounds__(MX_T) void mx_quantize_kernel(const void* __restrict__ x, long long ldx, long long rows, int K, int Kb, uint8_t* __restrict__ codes,
@@ -267,7 +268,8 @@ __device__ __forceinline__ void mx_decode32(const u32x4& c, float scale, float (
 }
 
 // One or two rows of x, K up to 128 KS: four lanes a row of W, a block of 32 each, against their 32 elements of x in registers -- 16 conversions and 32 M multiply-adds
-// for 16 bytes, under what memory delivers, and consecutive lanes read consecutive memory (in the matrix instruction's order they do not: see below).
+// for 16 bytes, under what memory delivers, and consecutive lanes read consecutive memory (in the matrix instruction's order they do not: see below).  1 x 786432 x 100 fp32:
+// 11.6 us for 48 MB (4.1 TB/s); what is left is the first loads' latency, behind x's way through LDS, and the tail.  768 to 2048 blocks differ by 4 %.
 template <int DT, int MM, int KS>
 __global__ __launch_bounds__(MX_T) void mx_linear_row_kernel(const MxLinear a) {
     const int lane = threadIdx.x & 63, b = lane & 3, r = lane >> 2;
@@ -364,6 +366,8 @@ __device__ __forceinline__ void mx_store_tile(const float* tile, void* y, long l
 
 // Any size: a block of four waves owns 64 NT rows of W and 16 CT rows of x; per 128 elements of K the x tile is cut into its pieces once, in LDS, in the
 // order in which the matrix instruction's lanes read it, and every wave multiplies its NT tiles of decoded W with it.
+// 256 x 15429 x 400: 11.2 us in bf16 (11 MB, 3.2 GFLOP), 21 in fp32 (three times the products); 16384 x 1024 x 1024 bf16: 50 us (0.7 PFLOP/s).  Bound by LDS: a step reads x's
+// pieces 16 bytes a lane for every NT products.  Loads two or four steps ahead of their use changed nothing (14.3 and 15.5 us where one step was 14.2).
 template <int DT, int NT, int CT>
 __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long long mtiles) {
     constexpr int P = mx_pieces<DT>(), NB = 64 * NT;
@@ -440,7 +444,7 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
 
 // Up to 16 rows of x and a long K (beyond what the kernels above hold of x): a block owns 32 rows of W and its eight waves share K, 128 elements at a time by turns, so that few
 // rows of W still give every CU work and a row is read 512 consecutive bytes at a time.  x goes from memory into the fragments, W as above; no barrier before the
-// waves' sums are joined, in order.
+// waves' sums are joined, in order.  1 x 4096 x 4096 bf16: 4.8 us (8.9 MB of W: latency), 8 x 4096 x 16384: 16 us (36 MB, 2.3 TB/s).
 constexpr int MX_LT = 512, MX_LN = 2;                            // threads; tiles of 16 rows of W
 template <int DT>
 __global__ __launch_bounds__(MX_LT) void mx_linear_long_kernel(const MxLinear a) {
@@ -514,7 +518,7 @@ struct MxInputGrad {
 };
 
 // One row of g, fp32: per 16 rows of W a lane decodes one block of 32 (four lanes a row) and adds it, times g, to its 32 sums -- 16 conversions and 32 M
-// multiply-adds for 16 bytes, under what memory delivers.
+// multiply-adds for 16 bytes, under what memory delivers.  1 x 786432 x 100: 11 us (45 MB, 4 TB/s), and 4 for the join.
 __global__ __launch_bounds__(MX_T) void mx_input_grad_row_kernel(const MxInputGrad a) {
     __shared__ float red[MX_T / 64][32][64 + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = lane & 3, r = lane >> 2;
@@ -563,6 +567,9 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_row_kernel(const MxInputGr
 // Any number of rows of g.  The sum runs along W's rows while its codes lie along K: a lane takes eight rows x eight elements of K (eight dwords), decodes them and turns
 // them in registers -- the bf16 pairs (k, k + 1) of two rows become the pairs (row, row + 1) of k and of k + 1 -- so that each of its eight k is one operand of a
 // matrix instruction over 32 rows.
+// 256 x 15429 x 400: 19 us in bf16 and 4 for the join (24.6 of 15424 columns of g, whose rows are aligned: 20); 64 x 786432 x 100: 39 us (142 MB, 3.6 TB/s).  A wave has few steps of 32
+// rows there, about 1 us each: bound by latency and the vector unit's decoding and turning (80 instructions for 32 products); loads two or three steps ahead: 24 and 23 us
+// where one step was 20; eight waves a block: no faster.
 template <int DT, int CT>
 __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a) {
     constexpr int P = mx_pieces<DT>(), WAVES = MX_T / 64;
@@ -745,6 +752,9 @@ struct MxMatmul {
 
 // A block of four waves owns BM rows of A x BN rows of B, a wave half of each (tiles of the scaled 16 x 16 x 128 instruction).  128 elements of K -- 64 bytes of codes and
 // four scale bytes a row -- go through LDS at a time, double-buffered, the next ones on their way in registers while these are multiplied.
+// 16384 x 1024 x 1024 to bf16: 21 us (1.6 PFLOP/s; 43 MB: 2 TB/s), 11 of them for what does not grow with K (x 128: 11.3 us), of which 34 MB of results are 6.  The loop takes
+// 1.5 us a step of 128, about twice its matrix instructions, LDS half of that; loads two or four steps ahead: 24.2 and 26.7 us where one step was 24.1.  Small ones are bound
+// by the launch (32 x 256 x 256: 3.4 us).
 constexpr int MM_Q = 4;       // blocks of 32 a step
 template <int ROWS>
 struct MxTile {
