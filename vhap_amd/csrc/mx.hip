@@ -180,7 +180,7 @@ __device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[
 __device__ __forceinline__ int mx_left(long long at, long long end) { return at >= end ? 0 : end - at < 8 ? (int)(end - at) : 8; }
 
 // ---- quantise / dequantise: four lanes a block, eight elements a lane (16 or 32 contiguous bytes of x, one dword of codes) ----
-// Bound by HBM: 786432 x 100 fp32 -> codes 64 us (356 MB, 5.6 TB/s), codes -> bf16 40 us (199 MB, 5.0 TB/s); small ones by the launch (1023 x 257: 2.5 us each).
+// Bound by HBM: 786432 x 100 fp32 -> codes 65 - 74 us (356 MB, 4.8 - 5.5 TB/s), codes -> bf16 38 - 41 us (199 MB, 5 TB/s); small ones by the launch (1023 x 257: 2.5 us each).
 // Index: unsigned where rows x blocks x 4 is below 2^31, long long beyond (a 64-bit division is a hundred instructions: 1000 x 1000 bf16 there and back 4.6 us / 4.9).
 template <int DT, typename Index>
 __global__ __launch_bounds__(MX_T) void mx_quantize_kernel(const void* __restrict__ x, long long ldx, long long rows, int K, int Kb, uint8_t* __restrict__ codes,
@@ -366,7 +366,7 @@ __device__ __forceinline__ void mx_store_tile(const float* tile, void* y, long l
 
 // Any size: a block of four waves owns 64 NT rows of W and 16 CT rows of x; per 128 elements of K the x tile is cut into its pieces once, in LDS, in the
 // order in which the matrix instruction's lanes read it, and every wave multiplies its NT tiles of decoded W with it.
-// 256 x 15429 x 400: 11.2 us in bf16 (11 MB, 3.2 GFLOP), 21 in fp32 (three times the products); 16384 x 1024 x 1024 bf16: 50 us (0.7 PFLOP/s).  Bound by LDS: a step reads x's
+// 256 x 15429 x 400: 11 - 14 us in bf16 (11 MB, 3.2 GFLOP), 21 in fp32 (three times the products); 16384 x 1024 x 1024 bf16: 50 us (0.7 PFLOP/s).  Bound by LDS: a step reads x's
 // pieces 16 bytes a lane for every NT products.  Loads two or four steps ahead of their use changed nothing (14.3 and 15.5 us where one step was 14.2).
 template <int DT, int NT, int CT>
 __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long long mtiles) {
