@@ -269,7 +269,8 @@ __device__ __forceinline__ void mx_decode32(const u32x4& c, float scale, float (
 
 // One or two rows of x, K up to 128 KS: four lanes a row of W, a block of 32 each, against their 32 elements of x in registers -- 16 conversions and 32 M multiply-adds
 // for 16 bytes, under what memory delivers, and consecutive lanes read consecutive memory (in the matrix instruction's order they do not: see below).  1 x 786432 x 100 fp32:
-// 11.6 us for 48 MB (4.1 TB/s); what is left is the first loads' latency, behind x's way through LDS, and the tail.  768 to 2048 blocks differ by 4 %.
+// 11.6 us for 48 MB (4.1 TB/s); what is left is the first loads' latency, behind x's way through LDS, and the tail.  768 to 2048 blocks differ by 4 %, and
+// the next rows read ahead of the products were no faster (12.4 us; 1 x 200000 x 400 20 instead of 13: their registers).
 template <int DT, int MM, int KS>
 __global__ __launch_bounds__(MX_T) void mx_linear_row_kernel(const MxLinear a) {
     const int lane = threadIdx.x & 63, b = lane & 3, r = lane >> 2;
