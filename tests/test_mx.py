@@ -497,3 +497,54 @@ def test_one_row_against_a_large_matrix(n, k):
     w.scales[n - 1, 0] = 255                                                     # the last row's first block alone
     dx = mx.linear_input_grad(g, w)
     assert dx[:, :32].isnan().all() and not dx[:, 32:].isnan().any()
+
+
+@pytest.mark.gpu
+def test_inference_mode_and_two_backwards():
+    w, x, g = random_mx(90, 70, 1), randn((4, 70), 2), randn((4, 90), 3)
+    want = mx.linear(x, w)
+    with torch.inference_mode():
+        assert torch.equal(mx.linear(x, w), want)
+        q = mx.quantize(x)
+        y = mx.matmul(q, w)
+        assert torch.equal(mx.linear(x.clone(), w), want)
+    assert torch.equal(y, mx.matmul(mx.quantize(x), w))
+    x1 = x.clone().requires_grad_()
+    y = mx.linear(x1, w)
+    y.backward(g, retain_graph=True)
+    first = x1.grad.clone()
+    y.backward(g)
+    assert torch.equal(x1.grad, first + first)
+    with pytest.raises(RuntimeError):
+        y.backward(g)
+    y = mx.linear(x1, w)                                                         # W changed between forward and backward: refused
+    w.codes.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(g)
+
+
+@pytest.mark.gpu
+def test_threads_and_streams_at_once():
+    """two host threads, each with its stream, on one matrix"""
+    import threading
+    w = random_mx(3000, 100, 1)
+    xs = [randn((m, 100), m) for m in (1, 7, 40, 1)]
+    want = [(mx.linear(x, w), mx.linear_input_grad(mx.linear(x, w), w)) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                x1 = xs[k].clone().requires_grad_()
+                y = mx.linear(x1, w)
+                y.backward(y.detach())
+                if not (torch.equal(y, want[k][0]) and torch.equal(x1.grad, want[k][1])):
+                    bad.append(k)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -229,6 +229,21 @@ def test_eager_step_with_clipped_gradients(flame_model):
     assert abs(n - 0.5) <= 0.5 * 2.0 ** -20
 
 
+@pytest.mark.gpu
+def test_an_optimiser_that_does_not_clip_by_itself(flame_model):
+    """a HipAdam made without the limit: the eager step clips in place ahead of it, the captured step (which updates inside its plan) refuses it"""
+    from vhap_amd.native import HipAdam
+    from vhap_amd.tracker import GraphedStep
+    tr, cfg = _tracker(flame_model, T=128, max_grad_norm=0.5)
+    made = tr.configure_optimizer(tr.get_train_parameters("rgb_global_tracking"))
+    opt = HipAdam([{"params": g["params"], "lr": g["lr"]} for g in made.param_groups])
+    tr.optimize_iter(tr.get_sample(np.arange(2)), opt, "rgb_global_tracking")
+    n = norm64([p.grad for g in opt.param_groups for p in g["params"] if p.grad is not None], 2.0)
+    assert abs(n - 0.5) <= 0.5 * 2.0 ** -20
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        GraphedStep(tr, tr.get_sample(np.arange(2), device_index=True), opt, "rgb_global_tracking", warmup=0)
+
+
 def test_clipping_on_the_host(flame_model):
     """a CPU tracker's landmark stage: torch's optimiser behind torch's clipping"""
     tr, cfg = _tracker(flame_model, device="cpu", T=64, H=32, W=32, max_grad_norm=0.25)

@@ -925,9 +925,9 @@ class GlobalTracker(FlameTracker):
         return log_dict
 
     def clip_gradients(self, optimizer):
-        """cfg.lr.max_grad_norm for an optimiser that does not clip by itself (HipAdam does, inside its update)"""
+        """cfg.lr.max_grad_norm for an optimiser that does not clip by itself (HipAdam(max_grad_norm=) does, inside its update)"""
         limit = self.cfg.lr.max_grad_norm
-        if limit is None or isinstance(optimizer, NV.HipAdam):
+        if limit is None or getattr(optimizer, "max_grad_norm", None) is not None:
             return
         params = [p for g in optimizer.param_groups for p in g["params"]]
         (NV.clip_grad_norm_ if str(self.device).startswith("cuda") else torch.nn.utils.clip_grad_norm_)(params, float(limit))
@@ -1319,6 +1319,8 @@ class GraphedStep:
         """`feed`: (dataloader stages over a resident FrameStore) let the captured step gather its own batch from an uploaded table --
         feed_upload() -- instead of being fed by the host between replays; see _enable_feed."""
         assert tracker.fused, "graph capture needs the fused (sync-free) path"
+        if tracker.cfg.lr.max_grad_norm is not None and isinstance(optimizer, NV.HipAdam) and optimizer.max_grad_norm is None:
+            raise ValueError("cfg.lr.max_grad_norm is set: a captured step clips inside its update, with HipAdam(max_grad_norm=) (what configure_optimizer makes)")
         self.feed, self._want_feed = None, bool(feed)
         self.defer_join, self._in_loop = False, False
         self.tr, self.opt, self.stage = tracker, optimizer, stage
