@@ -244,6 +244,22 @@ def test_an_optimiser_that_does_not_clip_by_itself(flame_model):
         GraphedStep(tr, tr.get_sample(np.arange(2), device_index=True), opt, "rgb_global_tracking", warmup=0)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("stage", ["lmk_init_all"])
+def test_captured_step_with_torchs_optimiser(flame_model, stage):
+    """torch.optim.Adam inside the captured native step: clipped in place ahead of it"""
+    from vhap_amd.tracker import GraphedStep
+    tr, cfg = _tracker(flame_model, T=128, max_grad_norm=1e-3)
+    made = tr.configure_optimizer(tr.get_train_parameters(stage))
+    opt = torch.optim.Adam([{"params": g["params"], "lr": g["lr"]} for g in made.param_groups], capturable=True)
+    st = GraphedStep(tr, tr.get_sample(np.arange(2), device_index=True), opt, stage, warmup=0)
+    for _ in range(3):
+        st()
+        torch.cuda.synchronize()
+        n = norm64([p.grad for p in st.params if p.grad is not None], 2.0)
+        assert abs(n - 1e-3) <= 1e-3 * 2.0 ** -18                                # (two roundings an element, and 1e-6 in the factor's denominator below 2^-18 of the norm)
+
+
 def test_clipping_on_the_host(flame_model):
     """a CPU tracker's landmark stage: torch's optimiser behind torch's clipping"""
     tr, cfg = _tracker(flame_model, device="cpu", T=64, H=32, W=32, max_grad_norm=0.25)

@@ -1408,6 +1408,7 @@ class GraphedStep:
                             ns.backward(1, optimizer=optimizer)
                         else:
                             ns.backward(1)
+                            tracker.clip_gradients(optimizer)
                             optimizer.step()
             elif not ns.photometric:
                 # Frame sharding of a landmark-only stage: forward, backward, ONE all-reduce of the (small) gradient arena, Adam
@@ -1417,6 +1418,7 @@ class GraphedStep:
                 with self.gB.capture(pool=self.gF.pool(), **cap):
                     ns.backward(world)
                 with self.gA.capture(pool=self.gF.pool(), **cap):
+                    tracker.clip_gradients(optimizer)
                     optimizer.step()
             else:
                 # Frame sharding.  The big collective is the texture gradient (50 MB at T = 2048).  The backward is captured in two plans:
@@ -1493,6 +1495,7 @@ class GraphedStep:
                             ns.tex_finish_rows(optimizer, self.tex_strip, self.tex_row0, self.tex_rows)      # (reads the step counter + 1 ...)
                             optimizer.step(skip=(tex,))                                                      # (... which this call then advances)
                         else:
+                            tracker.clip_gradients(optimizer)
                             optimizer.step()
             # Step k+1 under step k's texture tail: inside replay_stream() the single-GPU plan is replayed WITHOUT joining its side
             # streams at the end -- what it leaves open (the texture gradient's sort, tile pass, finish + Adam on the side stream) keeps
