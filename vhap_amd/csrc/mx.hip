@@ -368,7 +368,7 @@ __device__ __forceinline__ void mx_store_tile(const float* tile, void* y, long l
 // Any size: a block of four waves owns 64 NT rows of W and 16 CT rows of x; per 128 elements of K the x tile is cut into its pieces once, in LDS, in the
 // order in which the matrix instruction's lanes read it, and every wave multiplies its NT tiles of decoded W with it.
 // 256 x 15429 x 400: 11 - 14 us in bf16 (11 MB, 3.2 GFLOP), 21 in fp32 (three times the products); 16384 x 1024 x 1024 bf16: 50 us (0.7 PFLOP/s).  Bound by LDS: a step reads x's
-// pieces 16 bytes a lane for every NT products.  Loads two or four steps ahead of their use changed nothing (14.3 and 15.5 us where one step was 14.2).
+// pieces 16 bytes a lane for every NT products.  Loads two or three steps ahead of their use are slower (13.0 and 16.7 us where one step is 12.2).
 template <int DT, int NT, int CT>
 __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long long mtiles) {
     constexpr int P = mx_pieces<DT>(), NB = 64 * NT;
@@ -568,8 +568,8 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_row_kernel(const MxInputGr
 // Any number of rows of g.  The sum runs along W's rows while its codes lie along K: a lane takes eight rows x eight elements of K (eight dwords), decodes them and turns
 // them in registers -- the bf16 pairs (k, k + 1) of two rows become the pairs (row, row + 1) of k and of k + 1 -- so that each of its eight k is one operand of a
 // matrix instruction over 32 rows.
-// 256 x 15429 x 400: 19 us in bf16 and 4 for the join (24.6 of 15424 columns of g, whose rows are aligned: 20); 64 x 786432 x 100: 39 us (142 MB, 3.6 TB/s).  A wave has few steps of 32
-// rows there, about 1 us each: bound by latency and the vector unit's decoding and turning (80 instructions for 32 products); loads two or three steps ahead: 24 and 23 us
+// 256 x 15429 x 400: 19 us in bf16 and 4 for the join (4 of them because half of g's rows begin between two dwords: 20 in all for 15428 columns); 64 x 786432 x 100: 39 us (142 MB, 3.6 TB/s).  A wave has few steps of 32
+// rows there, about 1 us each: bound by latency and the vector unit's decoding and turning (80 instructions for 32 products); loads two or three steps ahead: 21 and 24 us
 // where one step was 20; eight waves a block: no faster.
 template <int DT, int CT>
 __global__ __launch_bounds__(MX_T) void mx_input_grad_kernel(const MxInputGrad a) {
