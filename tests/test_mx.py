@@ -548,3 +548,21 @@ def test_threads_and_streams_at_once():
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(4, 100, 1100), (1, 70, 2050), (40, 300, 200), (2, 40000, 200)])
+def test_not_finite_stays_where_it_is(m, n, k, dtype):
+    """a NaN block (the last of K, the last row), an infinity in x: only the results they enter"""
+    w = random_mx(n, k, 1, lo=124, hi=128)
+    w.scales[n - 1, -1] = 255
+    x = randn((m, k), 2, dtype)
+    y = mx.linear(x, w)
+    assert y[:, n - 1].isnan().all() and bool(y[:, :n - 1].isfinite().all())
+    x[m - 1, k - 1] = math.inf
+    y, last = mx.linear(x, w).cpu(), values64(w)[:, -1]
+    assert bool(y[:m - 1, :n - 1].isfinite().all())
+    row, last = y[m - 1, :n - 1], last[:n - 1]
+    assert bool((row.isnan() == (last == 0)).all())                              # infinity times zero
+    assert bool((row[last != 0] == (torch.sign(last[last != 0]) * math.inf).to(dtype)).all())
