@@ -362,8 +362,8 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
         return run_linear(x, codes, scales, N, K, bias ? *bias : Tensor());
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-        const Tensor& g = grads[0];
-        TORCH_CHECK(!(at::GradMode::is_enabled() && g.requires_grad()), "mx.linear is not twice differentiable");
+        TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].requires_grad()), "mx.linear is not twice differentiable");
+        const Tensor g = grads[0].resolve_neg();      // (autograd makes such views by itself: the imaginary part of a conjugate; what a user passes is refused)
         const auto saved = ctx->get_saved_variables();
         const int64_t N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt();
         Tensor dx, db;
