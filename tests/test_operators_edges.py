@@ -27,3 +27,14 @@ def test_a_gradient_that_is_a_negated_view(n):
     for of in (lambda y: y.backward(torch._neg_view(-c)), lambda y: (torch.complex(c, y).conj() * torch.complex(c, c)).real.sum().backward()):
         dx1, db1, seen = gradients(of)
         assert seen == [True] and torch.equal(dx1, dx) and torch.equal(db1, db)
+
+
+@pytest.mark.gpu
+def test_one_result_given_for_two_gradients():
+    """the first gradient goes through a copy, the second straight to the kernel"""
+    g = [randn((30, 40), 1).t(), randn((40, 30), 2)]
+    o, keep = randn((40, 30), 3), randn((40, 30), 3)
+    for grads in (g, g[::-1], [g[0], g[0]]):
+        with pytest.raises(ValueError, match="overlap|twice"):
+            NV.clip_by_global_norm(grads, 1.0, out=[o, o])
+        assert torch.equal(o, keep)

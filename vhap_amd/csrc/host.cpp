@@ -13,7 +13,6 @@
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
-#include <set>
 
 #include "vhap_hip.h"
 
@@ -191,7 +190,11 @@ py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
     c10::DeviceGuard guard(gs[0].device());
     // the kernels walk memory in order: a pair that is dense with the same strides is taken as it stands, anything else goes through contiguous copies
     Table t(gs.size());
-    std::vector<std::pair<Tensor, Tensor>> back;
+    struct Back {
+        Tensor to, from;
+        size_t place;                         // in the list
+    };
+    std::vector<Back> back;
     std::vector<Tensor> keep;
     for (size_t i = 0; i < gs.size(); i++) {
         const Tensor &g = gs[i], &o = outs[i];
@@ -204,21 +207,19 @@ py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
         const Tensor c = g.contiguous(), r = at::empty(c.sizes(), c.options());
         t.add(c, &r);
         keep.push_back(c);
-        back.emplace_back(o, r);
+        back.push_back({o, r, i});
     }
     if (!back.empty()) {                      // (dense ones among themselves: vhap_grad_clip sees to it)
         std::vector<std::pair<Place, size_t>> at;
         for (size_t i = 0; i < outs.size(); i++)
             if (outs[i].numel() > 0) at.emplace_back(Place(outs[i]), i);
         for (auto& b : back) {
-            if (b.first.numel() == 0) continue;
-            const Place mine(b.first);
+            if (b.to.numel() == 0) continue;
+            const Place mine(b.to);
             for (auto& x : at)
-                if (!b.first.is_same(outs[x.second]) && !mine.apart(x.first)) throw py::value_error("clipping: a strided result overlaps another result in memory");
+                if (x.second != b.place && !mine.apart(x.first))
+                    throw py::value_error("clipping: a strided result overlaps another result in memory (the same tensor twice in the list?)");
         }
-        std::set<const void*> once;
-        for (auto& b : back)
-            if (!once.insert(b.first.unsafeGetTensorImpl()).second) throw py::value_error("clipping: the same tensor twice in the list");
     }
     const size_t bytes = api.norm_bytes((int)gs.size());
     const Tensor ws = workspace(bytes, gs[0]), norm = at::empty({}, gs[0].options().dtype(at::kFloat));
@@ -226,7 +227,7 @@ py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
                             stream_of(norm));
     if (rc == VHAP_E_UNSUPPORTED) throw py::value_error("clipping: a result overlaps another result, or another gradient, in memory (the same tensor twice in the list?)");
     check(rc, "vhap_grad_clip");
-    for (auto& b : back) b.first.copy_(b.second);
+    for (auto& b : back) b.to.copy_(b.from);
     if (!made)
         for (const Tensor* o : outs.t)
             if (!o->is_inference()) o->unsafeGetTensorImpl()->bump_version();       // (written behind autograd's back)
