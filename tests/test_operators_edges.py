@@ -38,3 +38,66 @@ def test_one_result_given_for_two_gradients():
         with pytest.raises(ValueError, match="overlap|twice"):
             NV.clip_by_global_norm(grads, 1.0, out=[o, o])
         assert torch.equal(o, keep)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [60, 61])
+def test_results_that_interleave(width):
+    """no element in common, though each lies between the other's"""
+    buf = randn((40, width), 1, scale=3.0)
+    square = randn((50, 50), 2, scale=3.0)
+    cube = randn((6, 9, 8), 3, scale=3.0)
+    for whole, views in ((buf, [buf[:, ::2], buf[:, 1::2]]), (buf, [buf[::2], buf[1::2, ::3], buf[1::2, 1::3], buf[1::2, 2::3]]),
+                         (cube, [cube[:, ::3], cube[:, 1::3], cube[:, 2::3, ::2], cube[:, 2::3, 1::2]]), (buf.t(), [buf.t()[::3], buf.t()[1::3], buf.t()[2::3]])):
+        src = whole.clone()
+        _, norm = NV.clip_by_global_norm(views, 1.0, out=views)
+        want = norm64([src], 2)
+        assert near_norm(float(norm), want)
+        check_clipped(whole, src, coefficient(want, 1.0))
+    lines = [torch.diagonal(square), square.view(-1)[1::51]]
+    keep, src = square.clone(), [v.clone() for v in lines]
+    NV.clip_by_global_norm(lines, 1.0, out=lines)
+    for v, s in zip(lines, src):
+        check_clipped(v, s, coefficient(norm64(src, 2), 1.0))
+    rest = ~(torch.eye(50, dtype=torch.bool) | torch.diag(torch.ones(49, dtype=torch.bool), 1)).cuda()
+    assert torch.equal(square[rest], keep[rest])
+    for views in ([buf[:, ::2], buf[:, ::3]], [buf[::2], buf[::5, :1]], [square[:, :1], torch.diagonal(square)], [cube[:, :, ::3], cube[:, 8:, 6:7]]):
+        keep = [v.clone() for v in views]
+        with pytest.raises(ValueError, match="overlap"):
+            NV.clip_by_global_norm(views, 1.0, out=views)
+        assert all(torch.equal(v, k) for v, k in zip(views, keep))
+
+
+@pytest.mark.gpu
+def test_what_counts_as_overlapping_is_what_shares_memory():
+    """random strided pairs of both widths of element, against the sets of bytes"""
+    import random
+    rng = random.Random(5)
+    base = torch.zeros(1200, device="cuda")
+    taken = refused = 0
+    for _ in range(300):
+        views, bytes_of = [], []
+        for _ in range(2):
+            dt = rng.choice([torch.float32, torch.bfloat16])
+            sizes = [rng.randint(1, 4) for _ in range(rng.randint(1, 3))]
+            order, step, strides = list(range(len(sizes))), rng.randint(1, 3), [0] * len(sizes)
+            rng.shuffle(order)
+            for d in order:                                                      # (nested, so that no view overlaps itself)
+                strides[d] = step
+                step = step * sizes[d] + rng.randint(0, 5)
+            at = rng.randint(0, 40)
+            v = base.view(dt).as_strided(sizes, strides, at)
+            index = torch.arange(4800 // dt.itemsize).as_strided(sizes, strides, at).reshape(-1).tolist()
+            views.append(v)
+            bytes_of.append({i * dt.itemsize + b for i in index for b in range(dt.itemsize)})
+        grads = [torch.full(tuple(v.shape), 2.0, dtype=v.dtype, device="cuda") for v in views]
+        base.zero_()
+        if bytes_of[0] & bytes_of[1]:
+            refused += 1
+            with pytest.raises(ValueError, match="overlap"):
+                NV.clip_by_global_norm(grads, 1e9, out=views)
+        else:
+            taken += 1
+            NV.clip_by_global_norm(grads, 1e9, out=views)
+            assert all(bool((v == 2.0).all()) for v in views)
+    assert taken > 50 and refused > 50

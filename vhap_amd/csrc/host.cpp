@@ -12,6 +12,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "vhap_hip.h"
@@ -137,27 +138,55 @@ Tensor grad_norm(py::handle given, int kind) {
     return norm;
 }
 
-// Where a result lies: bytes [lo, hi), as runs of at most `run` bytes, `step` apart (the axis of the largest stride; step 0: a single run).
+// The bytes of a tensor: lo + sum c z over its axes (c: stride, 0 <= z <= most) and over the bytes of an element; all in [lo, hi).
 struct Place {
-    uintptr_t lo, hi, step, run;
+    struct Axis {
+        int64_t c, most;
+    };
+    int64_t lo, hi;
+    std::vector<Axis> axes;
     explicit Place(const Tensor& t) {
         const int64_t size = (int64_t)t.element_size();
-        int64_t outer = -1, all = 0;
+        lo = (int64_t)(uintptr_t)t.data_ptr();
+        hi = lo + size;
+        axes.push_back({1, size - 1});
         for (int64_t d = 0; d < t.dim(); d++) {
-            all += (t.size(d) - 1) * t.stride(d);
-            if (t.size(d) > 1 && (outer < 0 || t.stride(d) > t.stride(outer))) outer = d;
+            if (t.size(d) < 2 || t.stride(d) == 0) continue;
+            axes.push_back({t.stride(d) * size, t.size(d) - 1});
+            hi += axes.back().c * axes.back().most;
         }
-        lo = (uintptr_t)t.data_ptr();
-        hi = lo + (all + 1) * size;
-        step = outer < 0 ? 0 : t.stride(outer) * size;
-        run = outer < 0 ? size : hi - lo - (t.size(outer) - 1) * step;
     }
-    // nothing in common, as far as can be seen: apart, or (columns of one matrix) runs in different places of the same step
+    // Nothing in common.  lo + sum c z = b.lo + sum c' z', with z' counted from its other end, is sum c z + sum c' (most' - z') = b.hi - 1 - lo: one sum of positive
+    // steps that reaches a given place, or does not.
     bool apart(const Place& b) const {
         if (hi <= b.lo || b.hi <= lo) return true;
-        if (step == 0 || step != b.step) return false;
-        const uintptr_t to = b.lo >= lo ? (b.lo - lo) % step : (step - (lo - b.lo) % step) % step;
-        return to >= run && to + b.run <= step;
+        std::vector<Axis> all(axes);
+        all.insert(all.end(), b.axes.begin(), b.axes.end());
+        int steps = 20000;
+        return !reaches(all, b.hi - 1 - lo, steps);
+    }
+    // is there a z, 0 <= z_k <= most_k, with sum c_k z_k = place?  Largest c first, and only what the smaller ones can make up for: for axes that nest, two or three values
+    // each.  Yes where `steps` run out.
+    static bool reaches(std::vector<Axis>& axes, int64_t place, int& steps) {
+        std::sort(axes.begin(), axes.end(), [](const Axis& a, const Axis& b) { return a.c > b.c; });
+        size_t n = 0;
+        int64_t all = 0;
+        for (const Axis& a : axes) {          // (equal steps are one)
+            if (n > 0 && axes[n - 1].c == a.c) axes[n - 1].most += a.most;
+            else axes[n++] = a;
+            all += a.c * a.most;
+        }
+        axes.resize(n);
+        return search(axes, 0, place, all, steps);
+    }
+    static bool search(const std::vector<Axis>& axes, size_t k, int64_t place, int64_t all, int& steps) {       // all: the most that axes k, k + 1, ... add up to
+        if (place < 0 || place > all) return false;
+        if (place == 0 || place == all) return true;
+        if (--steps < 0) return true;
+        const int64_t c = axes[k].c, rest = all - c * axes[k].most;
+        for (int64_t z = std::min(axes[k].most, place / c); z >= 0 && place - c * z <= rest; z--)
+            if (search(axes, k + 1, place - c * z, rest, steps)) return true;
+        return false;
     }
 };
 
