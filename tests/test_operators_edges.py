@@ -101,3 +101,17 @@ def test_what_counts_as_overlapping_is_what_shares_memory():
             NV.clip_by_global_norm(grads, 1e9, out=views)
             assert all(bool((v == 2.0).all()) for v in views)
     assert taken > 50 and refused > 50
+
+
+@pytest.mark.gpu
+def test_a_result_that_overlaps_itself():
+    base = randn((64,), 1)
+    keep = base.clone()
+    for sizes, strides in (((5, 4), (1, 1)), ((4, 6), (5, 1)), ((3, 3, 3), (4, 2, 4)), ((7,), (0,))):
+        with pytest.raises(ValueError, match="share memory"):
+            NV.clip_by_global_norm([randn(sizes, 2)], 1.0, out=[base.as_strided(sizes, strides)])
+        assert torch.equal(base, keep)
+    g = randn((2, 3), 3)                                                         # 0, 2, 4, 3, 5, 7: strides that look as if they did
+    out = base.as_strided((2, 3), (3, 2))
+    NV.clip_by_global_norm([g], 1e9, out=[out])
+    assert torch.equal(out, g)

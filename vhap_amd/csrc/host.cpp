@@ -165,6 +165,21 @@ struct Place {
         int steps = 20000;
         return !reaches(all, b.hi - 1 - lo, steps);
     }
+    // Two of its own elements in one place: a difference of indices d, not zero, with sum c d = 0.  For each axis as the first with d_k > 0, c_k + c_k (d_k - 1) plus the later
+    // axes' c (d + most), 0 <= d + most <= 2 most, is the later axes' sum c most.
+    bool folded() const {
+        int steps = 20000;
+        for (size_t k = 1; k < axes.size(); k++) {
+            std::vector<Axis> rest{{axes[k].c, axes[k].most - 1}};
+            int64_t place = -axes[k].c;
+            for (size_t j = k + 1; j < axes.size(); j++) {
+                rest.push_back({axes[j].c, 2 * axes[j].most});
+                place += axes[j].c * axes[j].most;
+            }
+            if (reaches(rest, place, steps)) return true;
+        }
+        return false;
+    }
     // is there a z, 0 <= z_k <= most_k, with sum c_k z_k = place?  Largest c first, and only what the smaller ones can make up for: for axes that nest, two or three values
     // each.  Yes where `steps` run out.
     static bool reaches(std::vector<Axis>& axes, int64_t place, int& steps) {
@@ -231,8 +246,10 @@ py::tuple clip(py::handle given, py::object out, int kind, double max_norm) {
             t.add(g, &o);
             continue;
         }
-        for (int64_t d = 0; d < o.dim(); d++)
-            if (o.stride(d) == 0 && o.size(d) > 1) throw py::value_error(text(what, ": a result whose elements share memory (an expanded tensor)"));
+        bool shared = false;
+        for (int64_t d = 0; d < o.dim(); d++) shared |= o.stride(d) == 0 && o.size(d) > 1;
+        if (shared || (o.numel() > 1 && !o.is_non_overlapping_and_dense() && Place(o).folded()))
+            throw py::value_error(text(what, ": a result whose elements share memory (an expanded tensor, windows of one)"));
         const Tensor c = g.contiguous(), r = at::empty(c.sizes(), c.options());
         t.add(c, &r);
         keep.push_back(c);
