@@ -115,3 +115,27 @@ def test_a_result_that_overlaps_itself():
     out = base.as_strided((2, 3), (3, 2))
     NV.clip_by_global_norm([g], 1e9, out=[out])
     assert torch.equal(out, g)
+
+
+def test_a_forward_mode_tangent_is_refused():
+    """dropped, it would count as zero"""
+    import torch.autograd.forward_ad as fwAD
+    w, x, b, g = random_mx(70, 40, 1, "cpu"), torch.randn(5, 40), torch.randn(70), torch.randn(5, 70)
+    with fwAD.dual_level():
+        for call in (lambda: mx.linear(fwAD.make_dual(x, torch.ones_like(x)), w), lambda: mx.linear(x, w, fwAD.make_dual(b, torch.ones_like(b))),
+                     lambda: mx.linear_input_grad(fwAD.make_dual(g, torch.ones_like(g)), w)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
+@pytest.mark.gpu
+def test_a_forward_mode_tangent_is_refused_on_the_device():
+    import torch.autograd.forward_ad as fwAD
+    w, x, g = random_mx(70, 40, 1), randn((5, 40), 2), randn((5, 70), 3)
+    with fwAD.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+            mx.linear(fwAD.make_dual(x, torch.ones_like(x)), w)
+        x1 = x.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="forward-mode"):                  # forward over reverse
+            torch.autograd.grad(mx.linear(x1, w), x1, fwAD.make_dual(g, torch.ones_like(g)))
+        torch.autograd.grad(mx.linear(x1, w), x1, g)

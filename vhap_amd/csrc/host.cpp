@@ -331,8 +331,14 @@ void floats(const Tensor& t, const char* what) {
     plain(t, what);
 }
 
+// what a forward-mode tangent would be is the same product, but nothing here computes it: left out it would count as zero
+void no_tangent(const Tensor& t, const char* what) {
+    if (t._fw_grad(/*level=*/0).defined()) throw std::runtime_error(text(what, ": no forward-mode derivative (an input carries a tangent)"));
+}
+
 void pair_ok(const Tensor& x, const Tensor& codes, int64_t n, int64_t N, int64_t K, const char* what) {
     floats(x, what);
+    no_tangent(x, what);
     if (x.dim() < 1 || x.size(-1) != n) throw py::value_error(text(what, ": ", n, " elements along the last axis for a matrix of [", N, ", ", K, "], got ", x.sizes()));
     if (x.device() != codes.device()) throw py::value_error(text(what, ": tensors on one device, got ", x.device(), " and ", codes.device()));
     on_hip(x, what);
@@ -342,6 +348,7 @@ void bias_ok(const std::optional<Tensor>& bias, int64_t N, c10::Device device, c
     if (!bias) return;
     if (bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != N) throw py::value_error(text(what, ": a float32 bias of ", N, " elements"));
     plain(*bias, what);
+    no_tangent(*bias, what);
     if (bias->device() != device) throw py::value_error(text(what, ": the bias on ", device, ", got ", bias->device()));
 }
 
@@ -410,6 +417,7 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].requires_grad()), "mx.linear is not twice differentiable");
+        no_tangent(grads[0], "mx.linear's gradient");
         const Tensor g = grads[0].resolve_neg();      // (autograd makes such views by itself: the imaginary part of a conjugate; what a user passes is refused)
         const auto saved = ctx->get_saved_variables();
         const int64_t N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt();
@@ -432,8 +440,8 @@ void capture_ok(const Tensor& t, const char* what) {
 }
 
 Tensor linear(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t N, int64_t K, const std::optional<Tensor>& bias) {
-    pair_ok(x, codes, K, N, K, "linear");
     bias_ok(bias, N, x.device(), "linear");
+    pair_ok(x, codes, K, N, K, "linear");
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || (bias && bias->requires_grad()))) {
         at::NoGradGuard no_grad;
         return run_linear(x, codes, scales, N, K, bias ? *bias : Tensor());

@@ -122,14 +122,14 @@ def quantize_host(x):
 def linear(x, w, bias=None):
     """y [..., N] = x [..., K] w^T (+ bias): w an MXTensor [N, K], x float32 / bfloat16 / float16, bias float32 [N]; y in x's type.  The products are exact,
     the sums are float32 in a fixed order, y is rounded once (float32 numbers below 2^-117 lose their last bits, those below 2^-126 may count as 0).  Gradients
-    flow to x and bias (once: not twice differentiable).  In a stream capture, a differentiable call is refused while a graph of the same leaf made on another
-    stream is alive: its captured backward would end the process."""
+    flow to x and bias (once: not twice differentiable; an input with a forward-mode tangent is refused).  In a stream capture, a differentiable call is refused while
+    a graph of the same leaf made on another stream is alive: its captured backward would end the process."""
     N, K = _matrix(w, "linear")
     return _lib.host().linear(x, w.codes, w.scales, N, K, bias)
 
 
 def linear_input_grad(g, w):
-    """dx [..., K] = g [..., N] w for an MXTensor w [N, K]: the gradient of linear's input from that of its output, in g's type"""
+    """dx [..., K] = g [..., N] w for an MXTensor w [N, K]: the gradient of linear's input from that of its output, in g's type.  Not differentiable itself."""
     N, K = _matrix(w, "linear_input_grad")
     return _lib.host().input_grad(g, w.codes, w.scales, N, K)
 
