@@ -139,3 +139,85 @@ def test_a_forward_mode_tangent_is_refused_on_the_device():
         with pytest.raises(RuntimeError, match="forward-mode"):                  # forward over reverse
             torch.autograd.grad(mx.linear(x1, w), x1, fwAD.make_dual(g, torch.ones_like(g)))
         torch.autograd.grad(mx.linear(x1, w), x1, g)
+
+
+def _collectives(monkeypatch, seen):
+    """stand-ins for a group of two equal ranks over gloo: what they are given is noted"""
+    from vhap_amd import dist as D
+    monkeypatch.setattr(D.dist, "get_rank", lambda group=None: 0)
+    monkeypatch.setattr(D.dist, "get_world_size", lambda group=None: 2)
+    monkeypatch.setattr(D.dist, "get_backend", lambda group=None: "gloo")
+
+    def all_reduce(t, op=None, group=None, async_op=False):
+        seen.append(t)
+        t.mul_(2)
+
+    def all_gather_into_tensor(out, src, group=None, async_op=False):
+        seen.extend([out, src])
+        out.copy_(torch.cat([src, src]).view_as(out))
+    monkeypatch.setattr(D.dist, "all_reduce", all_reduce)
+    monkeypatch.setattr(D.dist, "all_gather_into_tensor", all_gather_into_tensor)
+    return D.FrameShardContext()
+
+
+def _use_collectives(ctx, make):
+    """every collective of the context on tensors from make(values) -> what they leave"""
+    v = torch.arange(24, dtype=torch.float32)
+    out = []
+    t = make(v)
+    out += [ctx.all_reduce_sum(t), t]
+    t = make(v)
+    assert ctx.all_reduce_sum_(t) is t
+    out.append(t)
+    for a in (False, True):
+        t = make(v)
+        w = ctx.all_reduce_mean_(t, async_op=a)
+        assert w is None
+        full, part = make(v), make(torch.zeros(12))
+        ctx.reduce_scatter_mean(full, part, async_op=a).wait()
+        planes = make(v.view(3, 4, 2))
+        for w in ctx.all_gather_rows(planes, 0, 2, async_op=a):
+            w.wait()
+        out += [t, part, planes]
+    p, q = make(v).requires_grad_(), make(v[:5]).requires_grad_()
+    p.grad = make(v * 3)
+    ctx.average_gradients([p, q])
+    return out + [p.grad, q.grad]
+
+
+def _check_collectives(out):
+    v = torch.arange(24, dtype=torch.float32)
+    planes = v.view(3, 4, 2)
+    gathered = torch.cat([planes[:, :2], planes[:, :2]], 1)
+    want = [2 * v, v, 2 * v] + [v, v[:12], gathered] * 2 + [3 * v, torch.zeros(5)]
+    assert len(out) == len(want)
+    for a, b in zip(out, want):
+        assert a.shape == b.shape and torch.equal(a.detach().cpu(), b)
+
+
+class _Elsewhere(torch.Tensor):
+    """a tensor in host memory that says it is on the device"""
+    is_cuda = True
+
+    def cpu(self):
+        return self.detach().as_subclass(torch.Tensor).clone()
+
+
+def test_gloo_is_given_host_memory(monkeypatch):
+    seen = []
+    ctx = _collectives(monkeypatch, seen)
+    out = _use_collectives(ctx, lambda v: v.clone().as_subclass(_Elsewhere))
+    assert len(seen) > 10 and not any(isinstance(t, _Elsewhere) for t in seen)
+    _check_collectives([t.as_subclass(torch.Tensor) for t in out])
+    seen.clear()
+    _check_collectives(_use_collectives(ctx, lambda v: v.clone()))               # and what is in host memory goes as it is
+    assert len(seen) > 10
+
+
+@pytest.mark.gpu
+def test_gloo_is_given_host_memory_of_device_tensors(monkeypatch):
+    seen = []
+    ctx = _collectives(monkeypatch, seen)
+    out = _use_collectives(ctx, lambda v: v.cuda())
+    assert len(seen) > 10 and not any(t.is_cuda for t in seen) and all(t.is_cuda for t in out)
+    _check_collectives(out)

@@ -13,7 +13,8 @@ The eager `optimize_iter` averages one flat bucket of all gradients instead (`av
 The per-rank energy is defined so that its mean over ranks equals the single-GPU energy (equal shards): batch means become local
 means, the photometric numerator is multiplied by world_size through the normaliser.  Replicas stay bit-identical because every rank
 applies the same averaged gradient with the same Adam state.  The colour disturbance draws its pools from the local shard only.
-Backend: 'nccl' (= RCCL over xGMI on ROCm) on GPUs, 'gloo' in the CPU tests.
+Backend: 'nccl' (= RCCL over xGMI on ROCm) on GPUs, 'gloo' in the CPU tests and where several ranks share one GPU: it is given host memory only, device
+tensors go through a synchronous copy there and back (its collectives on device tensors can hang when ranks share a GPU).
 """
 import os
 
@@ -112,13 +113,16 @@ class FrameShardContext:
 
     # ---- collectives ----
     def all_reduce_sum(self, t):
-        t = t.clone()
-        dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group)
-        return t
+        return self.all_reduce_sum_(t.clone())
 
     def all_reduce_sum_(self, t):
         """in place (no clone): t = sum over ranks of t"""
-        dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group)
+        if t.is_cuda and dist.get_backend(self.group) != "nccl":
+            host = t.cpu()                                        # (waits for the current stream)
+            dist.all_reduce(host, op=dist.ReduceOp.SUM, group=self.group)
+            t.copy_(host)
+        else:
+            dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group)
         return t
 
     def broadcast_int(self, value, src=0):
@@ -135,8 +139,7 @@ class FrameShardContext:
         if dist.get_backend(self.group) == "nccl":
             work = dist.all_reduce(t, op=dist.ReduceOp.AVG, group=self.group, async_op=async_op)
             return work if async_op else None
-        dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group)
-        t.mul_(1.0 / self.world_size)
+        self.all_reduce_sum_(t).mul_(1.0 / self.world_size)
         return None
 
     class _Done:
@@ -153,7 +156,7 @@ class FrameShardContext:
         if dist.get_backend(self.group) == "nccl":
             work = dist.reduce_scatter_tensor(out, full, op=dist.ReduceOp.AVG, group=self.group, async_op=async_op)
             return work if async_op else self._Done()
-        dist.all_reduce(full, op=dist.ReduceOp.SUM, group=self.group)
+        self.all_reduce_sum_(full)
         out.copy_(full.view(n, -1)[self.rank].view_as(out)).mul_(1.0 / n)
         return self._Done()
 
@@ -168,6 +171,12 @@ class FrameShardContext:
             # RCCL gathers IN PLACE when the input is the rank's own slot of the output (sendbuff == recvbuff + rank * count): no staging
             # copy of the strip; gloo is handed a copy
             src = planes[c, row0:row0 + nrows]
+            if not nccl and planes.is_cuda:
+                host = torch.empty(planes[c].shape, dtype=planes.dtype)
+                dist.all_gather_into_tensor(host, src.cpu(), group=self.group)
+                planes[c].copy_(host)
+                works.append(self._Done())
+                continue
             if not nccl:
                 src = src.clone()
             w = dist.all_gather_into_tensor(planes[c], src, group=self.group, async_op=async_op)
@@ -190,8 +199,7 @@ class FrameShardContext:
             else:
                 flat[o:o + n].copy_(p.grad.reshape(-1))
             o += n
-        dist.all_reduce(flat, op=dist.ReduceOp.SUM, group=self.group)
-        flat.mul_(1.0 / self.world_size)
+        self.all_reduce_sum_(flat).mul_(1.0 / self.world_size)
         o = 0
         for p in params:
             n = p.numel()
