@@ -221,3 +221,34 @@ def test_gloo_is_given_host_memory_of_device_tensors(monkeypatch):
     out = _use_collectives(ctx, lambda v: v.cuda())
     assert len(seen) > 10 and not any(t.is_cuda for t in seen) and all(t.is_cuda for t in out)
     _check_collectives(out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 130, 70), (2, 40000, 150), (1, 40000, 300), (4, 100, 70), (40, 300, 135), (40, 20000, 20), (33, 70000, 33), (3, 40, 1030), (16, 100, 1100)])
+def test_codes_behind_the_last_element_are_no_numbers(m, n, k, dtype):
+    """the largest scales, at which a code of 4 or 6 (253) or of 2 and more (254) is past float32: elements that are not, codes behind them that are"""
+    w = random_mx(n, k, 1, lo=253, hi=255)
+    kb = w.scales.shape[1]
+    half = torch.randint(0, 2, (n, 32 * kb), generator=torch.Generator().manual_seed(2), dtype=torch.uint8) + 8 * torch.randint(
+        0, 2, (n, 32 * kb), generator=torch.Generator().manual_seed(3), dtype=torch.uint8)                      # +-0, +-0.5
+    half[:, k:] = 7
+    w.codes.copy_((half[:, 0::2] | half[:, 1::2] << 4).cuda())
+    W, X = values64(w), (randn((m, k), 4) * 2.0 ** -12).to(dtype)
+    X64 = X.cpu().double()
+    want, mags = X64 @ W.t(), X64.abs() @ W.abs().t()
+    got = mx.linear(X, w)
+    if dtype == torch.float16:
+        assert not bool(got.isnan().any())                                       # (infinite: past float16)
+    else:
+        assert float(mags.max()) < 3.4e38
+        check_sum(got, want, mags, k * PIECES[dtype], dtype)
+
+
+@pytest.mark.gpu
+def test_matmul_with_codes_behind_the_last_element_at_the_largest_scales():
+    for m, n, k in ((40, 50, 70), (6200, 1000, 70)):
+        a, b = random_mx(m, k, 1, lo=253, hi=255, garbage=True), random_mx(n, k, 2, lo=60, hi=64, garbage=True)
+        A, B = values64(a), values64(b)
+        check_sum(mx.matmul(a, b), A @ B.t(), A.abs() @ B.abs().t(), k, torch.float32)
+        check_sum(mx.matmul(b, a), B @ A.t(), B.abs() @ A.abs().t(), k, torch.float32)

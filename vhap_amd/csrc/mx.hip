@@ -42,11 +42,19 @@ __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_floa
 
 // the 16 bytes of codes and the scale byte of block `blk` of `row`; behind the last row or block: the last one's, without a branch around the load.  Nothing is wrong with that
 // where the other operand is zero behind the last block (or row, in the input's gradient) and results behind the last row are not stored: a product with zero is
-// zero, or NaN where that last block is NaN and the sum is NaN already.
+// zero, or not finite where that last block is not and the sum is not already -- by its elements: the codes behind K, which may be anything and past float32 by their scale, are
+// masked where they are multiplied (mx_masks).
 __device__ __forceinline__ u32x4 mx_block(const MxMatrix& w, long long row, int blk, unsigned& scale) {
     const size_t at = (size_t)min(row, w.rows - 1) * w.Kb + min(blk, w.Kb - 1);
     scale = w.scales[at];
     return reinterpret_cast<const u32x4*>(w.codes)[at];
+}
+
+// which bits of eight codes are elements, `left` of them and more from the first on; of a block's four dwords
+__device__ __forceinline__ unsigned mx_mask(int left) { return left >= 8 ? ~0u : left <= 0 ? 0u : (1u << 4 * left) - 1u; }
+__device__ __forceinline__ void mx_masks(int left, unsigned (&mask)[4]) {
+#pragma unroll
+    for (int d = 0; d < 4; d++) mask[d] = mx_mask(left - 8 * d);
 }
 
 __device__ __forceinline__ unsigned mx_pair_bits(bf16x2 v) { return __builtin_bit_cast(unsigned, v); }
@@ -335,6 +343,38 @@ __global__ __launch_bounds__(MX_T) void mx_linear_row_kernel(const MxLinear a) {
                 mine[m] = t == 0 ? sum[m] : b == t ? sum[m] : mine[m];
             }
         }
+        // A NaN may come from a code behind K that its scale puts past float32, times zero: then, and only then, these rows' products are formed again with such codes masked
+        // (masking every block cost 2 - 5 % of the kernel, and at KS = 4 the registers of half of its waves)
+        bool bad = false;
+#pragma unroll
+        for (int m = 0; m < MM; m++) bad |= mine[m] != mine[m];
+        if (a.w.K % 32 && __any(bad)) {
+#pragma unroll 1
+            for (int t = 0; t < 4; t++) {
+                float sum[MM];
+#pragma unroll
+                for (int m = 0; m < MM; m++) sum[m] = 0.f;
+#pragma unroll 1
+                for (int i = 0; i < 4 * KS; i++) {                // eight codes at a time, x out of LDS
+                    const int blk = (i & ~3) + b, k = 32 * blk + 8 * (i & 3), left = a.w.K - k;
+                    const unsigned at = (unsigned)(min(16 * t + r, last) * a.w.Kb + min(blk, a.w.Kb - 1));
+                    const unsigned w8 = reinterpret_cast<const unsigned*>(gc)[4 * (size_t)at + (i & 3)] & mx_mask(left);
+                    const float sc = mx_scale(gs[at]);
+                    const f32x2 w[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w8, sc, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w8, sc, 1),
+                                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w8, sc, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w8, sc, 3)};
+#pragma unroll
+                    for (int m = 0; m < MM; m++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) sum[m] = fmaf(w[e >> 1][e & 1], xs[m][k + e], sum[m]);
+                }
+#pragma unroll
+                for (int m = 0; m < MM; m++) {
+                    sum[m] += vhap_dpp<0xB1>(sum[m]);
+                    sum[m] += vhap_dpp<0x4E>(sum[m]);
+                    if (b == t && mine[m] != mine[m]) mine[m] = sum[m];
+                }
+            }
+        }
 #pragma unroll
         for (int m = 0; m < MM; m++)
             if (m < a.M && n < a.w.rows) mx_put<DT>(a.y, m * a.w.rows + n, a.bias ? mine[m] + bias : mine[m]);
@@ -410,6 +450,12 @@ __global__ __launch_bounds__(MX_T) void mx_linear_kernel(const MxLinear a, long 
             for (int p = 0; p < P; p++) xs[ct][tid & 3][p][((tid & 15) >> 2) * 16 + (xr ^ (tid & 3) << 2)] = f[p];   // (16 neighbouring lanes: 16 places modulo 256 bytes)
         }
         bf16x8 w[NT][4];
+        if (128 * ks + 128 > a.w.K) {                                        // (the last step, where it ends inside)
+            unsigned mask[4];
+            mx_masks(a.w.K - 128 * ks - 32 * (lane & 3), mask);
+#pragma unroll
+            for (int t = 0; t < NT; t++) c[t] &= u32x4{mask[0], mask[1], mask[2], mask[3]};
+        }
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const float sc = mx_scale((unsigned)__builtin_amdgcn_ds_bpermute(from, (int)s[t]));
@@ -474,6 +520,12 @@ __global__ __launch_bounds__(MX_LT) void mx_linear_long_kernel(const MxLinear a)
         for (int j = 0; j < 4; j++) {
             mx_settle8<DT>(a.x, xrow, 128 * ks + 32 * q + 8 * j, a.w.K, xv[j]);
             mx_fragments<DT>(xv[j], x[j]);
+        }
+        if (128 * ks + 128 > a.w.K) {
+            unsigned mask[4];
+            mx_masks(a.w.K - 128 * ks - 32 * (lane & 3), mask);
+#pragma unroll
+            for (int t = 0; t < MX_LN; t++) c[t] &= u32x4{mask[0], mask[1], mask[2], mask[3]};
         }
 #pragma unroll
         for (int t = 0; t < MX_LN; t++) {
@@ -850,8 +902,7 @@ __global__ __launch_bounds__(MX_T, 4) void mx_matmul_kernel(const MxMatmul a, lo
         if constexpr (!WHOLE) {
             const int left = k + blk < Kb - 1 ? 32 : k + blk == Kb - 1 ? (last ? last : 32) : 0;
             unsigned mask[4];
-#pragma unroll
-            for (int d = 0; d < 4; d++) mask[d] = left >= 8 * d + 8 ? ~0u : left <= 8 * d ? 0u : (1u << 4 * (left - 8 * d)) - 1u;
+            mx_masks(left, mask);
 #pragma unroll
             for (int h = 0; h < CB; h++) { cb[h].x &= mask[0]; cb[h].y &= mask[1]; cb[h].z &= mask[2]; cb[h].w &= mask[3]; }
             const int there = min(Kb - k, 4);                     // blocks of this step that exist; the others: scale 1
