@@ -913,7 +913,7 @@ int vhap_nhwc_add(const float* a, const float* b, const float* c, long long n, f
  *     halves to the even code; a block with a NaN or an infinity becomes NaN.
  *   vhap_mx4_dequantize: out [rows, K] contiguous (float32 and bfloat16 hold every value exactly; float16 rounds, and overflows above 65504).
  *   vhap_mx4_linear: y [M, N] = x [M, K] W^T + bias; W [N, K] in 4 bits, bias float32 [N] or NULL; x and y of `dtype`, products exact, sums in float32.
- *   vhap_mx4_linear_input_grad: dx [M, K] = g [M, N] W, N > 0; workspace of _workspace_bytes(M, N, K), partial sums joined in a fixed order;
+ *   vhap_mx4_linear_input_grad: dx [M, K] = g [M, N] W, N > 0; workspace of _workspace_bytes(M, N, K), partial sums joined in a fixed order (16 bytes where the sum is not split);
  *     VHAP_CALL_MX_ACCUMULATE (float32): dx += .   vhap_mx4_column_sums: out [N] = sum over the M rows of g (the bias' gradient).
  *   vhap_mx4_matmul: y [M, N] = A [M, K] B [N, K]^T + bias, both in 4 bits; VHAP_CONV_OUT_RELU: ReLU on the way out (a pointwise convolution: M pixels).
  * Empty results are VHAP_OK without a launch.

@@ -252,3 +252,28 @@ def test_matmul_with_codes_behind_the_last_element_at_the_largest_scales():
         A, B = values64(a), values64(b)
         check_sum(mx.matmul(a, b), A @ B.t(), A.abs() @ B.abs().t(), k, torch.float32)
         check_sum(mx.matmul(b, a), B @ A.t(), B.abs() @ A.abs().t(), k, torch.float32)
+
+
+def test_a_gradient_that_needs_no_partial_sums_asks_for_next_to_no_workspace():
+    bytes_of = _lib.lib().vhap_mx4_linear_input_grad_workspace_bytes
+    assert 0 < bytes_of(4_200_000, 8, 33) <= 64 and 0 < bytes_of(5, 300, 90) <= 64
+    assert bytes_of(1, 786432, 100) >= 4 * 128 * 256 and bytes_of(256, 15429, 400) >= 4 * 2 * 256 * 512
+    assert bytes_of(1, 1 << 20, 7) >= 4 * 128 and bytes_of(1, 2, (1 << 24)) >= 4 * (1 << 24)     # one row against many blocks: always by way of partial sums
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_gradient_without_partial_sums(dtype):
+    L, w, g = _lib.lib(), random_mx(300, 90, 1), randn((5, 300), 2, dtype)
+    dx, code, ws = torch.empty(5, 90, dtype=dtype, device="cuda"), TYPES.index(dtype), torch.empty(64, dtype=torch.uint8, device="cuda")
+    _lib.check(L.vhap_mx4_linear_input_grad(g.data_ptr(), code, 300, 5, w.codes.data_ptr(), w.scales.data_ptr(), 300, 90, ws.data_ptr(), 64, dx.data_ptr(), 0,
+                                            torch.cuda.current_stream().cuda_stream), "vhap_mx4_linear_input_grad")
+    W, G = values64(w), g.cpu().double()
+    check_sum(dx, G @ W, G.abs() @ W.abs(), 300 * PIECES[dtype], dtype)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    m = 200_000                                                                  # dx alone is 18 MB, partial sums would be 102
+    mx.linear_input_grad(torch.zeros(m, 8, dtype=dtype, device="cuda"), random_mx(8, 45, 1))
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 1.2 * m * (8 + 45) * dtype.itemsize + (4 << 20)

@@ -1137,6 +1137,7 @@ extern "C" size_t vhap_mx4_linear_input_grad_workspace_bytes(long long M, long l
     if (!mx_dims(N, K) || !mx_dims(M, K) || M == 0 || N == 0) return 0;
     // (the types differ in their splits: bf16 has the largest tiles and so the most splits, except where an fp32 row goes its own way)
     const GradPlan p = mx_grad_plan(M, N, K, VHAP_DTYPE_BF16), row = mx_grad_plan(M, N, K, VHAP_DTYPE_F32);
+    if (p.splits == 1 && !row.row) return 4 * sizeof(float);     // (one split is stored as the result; never none, so that a workspace can always be asked for and given)
     return sizeof(float) * (size_t)std::max(p.splits, row.splits) * (size_t)M * 128 * (size_t)p.ktiles;
 }
 
