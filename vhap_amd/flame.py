@@ -201,8 +201,8 @@ class FlameTexPCA(nn.Module):
         S = self.src_size
         if self.basis_format == "fp32":
             texture = self.texture_mean + (self.texture_basis * texcode[:, None, :]).sum(-1)
-        elif texcode.is_cuda:
-            texture = mx.linear(texcode, self.mx_basis(), self.texture_mean.reshape(-1))
+        elif texcode.is_cuda and texcode.dtype in mx.DTYPES:
+            texture = mx.linear(texcode, self.mx_basis(), self.texture_mean.reshape(-1).float())           # (the module may have been moved to another type)
         else:
             texture = self.texture_mean.reshape(1, -1) + texcode @ self.mx_basis().dequantize(torch.float32).to(texcode.dtype).t()
         texture = texture.reshape(texcode.shape[0], S, S, 3).permute(0, 3, 1, 2)

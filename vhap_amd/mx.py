@@ -18,7 +18,7 @@ import torch
 from . import _lib
 
 BLOCK = 32
-_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 class MXTensor:
@@ -67,7 +67,7 @@ class MXTensor:
 
     def dequantize(self, dtype=torch.float32):
         """the numbers as float32 or bfloat16 (both hold them exactly) or float16 (which rounds, and overflows above 65504)"""
-        if dtype not in _DTYPES:
+        if dtype not in DTYPES:
             raise TypeError(f"dequantize to float32, bfloat16 or float16, got {dtype}")
         K = self.shape[-1]
         if self.codes.is_cuda:
@@ -96,7 +96,7 @@ def quantize(x):
 
 def quantize_host(x):
     """quantize of a CPU tensor, in torch operations, to the same codes and scales (a model's constants are laid out once, before they move to the device)"""
-    if x.dtype not in _DTYPES:
+    if x.dtype not in DTYPES:
         raise TypeError(f"quantize_host: a float32, bfloat16 or float16 tensor, got {x.dtype}")
     if x.is_cuda or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"quantize_host: a CPU tensor with at least one element along the last axis, got {tuple(x.shape)} on {x.device}")
@@ -142,6 +142,6 @@ def matmul(a, b, bias=None, relu=False, out_dtype=torch.float32):
         raise ValueError(f"matmul: operands of one K, got {tuple(a.shape)} and {tuple(b.shape)}")
     if a.codes.device != b.codes.device:
         raise ValueError(f"matmul: tensors on one device, got {a.device} and {b.device}")
-    if out_dtype not in _DTYPES:
+    if out_dtype not in DTYPES:
         raise TypeError(f"matmul to float32, bfloat16 or float16, got {out_dtype}")
     return _lib.host().matmul(a.codes, a.scales, b.codes, b.scales, M, N, K, bias, relu, out_dtype)
