@@ -302,3 +302,14 @@ def test_the_texture_space_in_other_types(dtype):
     assert bool(((out.detach().cpu().double() - want.clamp(0, 1)).abs() <= limit).all())
     out.sum().backward()
     assert code.grad.dtype == dtype and bool(code.grad.isfinite().all()) and bool(code.grad.any())
+
+
+def test_a_limit_that_is_no_limit_is_refused_on_the_host(flame_model):
+    """torch's clipping takes a negative limit and turns the gradients round"""
+    from tests.test_operators_in_use import _tracker
+    import numpy as np
+    for bad in (-1.0, math.nan):
+        tr, _ = _tracker(flame_model, device="cpu", T=64, H=32, W=32, max_grad_norm=bad)
+        with pytest.raises(ValueError, match="max_norm"):
+            opt = tr.configure_optimizer(tr.get_train_parameters("lmk_init_all"))
+            tr.optimize_iter(tr.get_sample(np.arange(2)), opt, "lmk_init_all")

@@ -392,7 +392,8 @@ def _norm_kind(norm_type):
     return kind
 
 
-def _max_norm(v):
+def largest_norm(v):
+    """a limit on a norm as a float, refused where it is none"""
     v = float(v)
     if not v >= 0.0:
         raise ValueError(f"max_norm must not be negative or NaN, got {v}")
@@ -411,14 +412,14 @@ def clip_by_global_norm(grads, max_norm, norm_type=2.0, out=None):
     left alone), or memory that overlaps none of them; None: new tensors.  No synchronisation."""
     grads = _tensors(grads)
     out = grads if out is grads else out if out is None else _tensors(out)
-    return _lib.host().clip(grads, out, _norm_kind(norm_type), _max_norm(max_norm))
+    return _lib.host().clip(grads, out, _norm_kind(norm_type), largest_norm(max_norm))
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ on the HIP device: the gradients of `parameters` scaled in place to a global norm of at most max_norm; returns the
     norm they had, a 0-dim float32 tensor.  Parameters without a gradient are skipped.  `error_if_nonfinite`: raise before anything is scaled where the norm
     is NaN or infinite (waits for the device: not in a capture)."""
-    max_norm, kind = _max_norm(max_norm), _norm_kind(norm_type)
+    max_norm, kind = largest_norm(max_norm), _norm_kind(norm_type)
     ps = [parameters] if torch.is_tensor(parameters) else list(parameters)
     gs = [p.grad for p in ps if p.grad is not None]
     if not gs:
@@ -444,7 +445,7 @@ class HipAdam(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, max_grad_norm=None):
         if max_grad_norm is not None:
-            max_grad_norm = _max_norm(max_grad_norm)
+            max_grad_norm = largest_norm(max_grad_norm)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps))
         self.max_grad_norm = max_grad_norm
         self.grad_norm = None

@@ -929,8 +929,9 @@ class GlobalTracker(FlameTracker):
         limit = self.cfg.lr.max_grad_norm
         if limit is None or getattr(optimizer, "max_grad_norm", None) is not None:
             return
+        limit = NV.largest_norm(limit)                            # (torch's clipping takes a negative one and turns the gradients round)
         params = [p for g in optimizer.param_groups for p in g["params"]]
-        (NV.clip_grad_norm_ if str(self.device).startswith("cuda") else torch.nn.utils.clip_grad_norm_)(params, float(limit))
+        (NV.clip_grad_norm_ if str(self.device).startswith("cuda") else torch.nn.utils.clip_grad_norm_)(params, limit)
 
     def initialize_next_timtestep(self, timesteps):
         """tracker.py:1515-1529 (including its skip of the last frame)."""
