@@ -1067,8 +1067,7 @@ int mx_linear_launch(const MxLinear& a, hipStream_t st) {
     if (tiles > MX_MOST_BLOCKS) return VHAP_E_BADDIM;
 #define MX_LINEAR(NT, CT) mx_linear_kernel<DT, NT, CT><<<(int)tiles, MX_T, 0, st>>>(a, mtiles)
     if (two) { if (nt == 4) MX_LINEAR(4, 2); else MX_LINEAR(2, 2); }
-    else if (nt == 4) MX_LINEAR(4, 1);
-    else if (nt == 2) MX_LINEAR(2, 1);
+    else if (nt == 2) MX_LINEAR(2, 1);                           // (16 rows of x: fewer than 512 tiles, so never 256 rows of W)
     else MX_LINEAR(1, 1);
 #undef MX_LINEAR
     VHAP_LAUNCH_CHECK();
