@@ -313,3 +313,28 @@ def test_a_limit_that_is_no_limit_is_refused_on_the_host(flame_model):
         with pytest.raises(ValueError, match="max_norm"):
             opt = tr.configure_optimizer(tr.get_train_parameters("lmk_init_all"))
             tr.optimize_iter(tr.get_sample(np.arange(2)), opt, "lmk_init_all")
+
+
+@pytest.mark.gpu
+def test_a_capture_beside_an_eager_graph_behind_the_input():
+    """x made in the capture from a leaf of which an eager graph is alive, x itself made outside; nothing of either is differentiated here"""
+    w = random_mx(70, 40, 1)
+    leaf = randn((5, 40), 2).requires_grad_()
+    bias = randn((70,), 3).requires_grad_()
+    alive = [leaf * 2, bias * 2]
+    torch.cuda.synchronize()
+    for call in (lambda: mx.linear(leaf * 3, w), lambda: mx.linear(alive[0], w), lambda: mx.linear(torch.ones(5, 40, device="cuda"), w, bias * 3),
+                 lambda: mx.linear((leaf * 3).view(5, 40)[:, :40] + 1, w)):
+        with pytest.raises(RuntimeError, match="alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    del alive
+    torch.cuda.synchronize()
+    graph, g = torch.cuda.CUDAGraph(), randn((5, 70), 4)
+    with torch.cuda.graph(graph):
+        dx, db = torch.autograd.grad(mx.linear(leaf * 3, w, bias * 1), (leaf, bias), g)
+    for k in range(3):
+        g.copy_(randn((5, 70), 10 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, 3 * mx.linear_input_grad(g, w)) and torch.equal(db, torch.autograd.grad(mx.linear(leaf.detach(), w, b1 := bias.detach().clone().requires_grad_()), b1, g)[0])

@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <unordered_set>
 
 #include "vhap_hip.h"
 
@@ -428,15 +429,28 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
     }
 };
 
-// A leaf's gradient node keeps the stream it was made on for as long as any graph holds it.  One made outside a capture would make the captured backward wait for that
-// stream, which a capture does not survive (the runtime ends the process): said here, while it can be.
+// A node keeps the stream it was made on, a leaf's gradient node for as long as any graph holds it.  One made outside a capture makes the captured backward wait for that
+// stream; where it is the default stream, that is nothing a capture survives (the runtime ends the process), wherever behind the input it lies.  Said here, while it can
+// be.  (Other streams join the capture and leave it again; for the input's own node they are refused too.)
 void capture_ok(const Tensor& t, const char* what) {
-    if (!t.requires_grad() || !t.is_leaf()) return;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!node) return;
-    const auto made_on = node->stream();
-    if (made_on && made_on->id() != c10::hip::getCurrentHIPStream(t.device().index()).id())
-        throw std::runtime_error(text(what, ": in a stream capture, while a graph of the same leaf made on another stream is alive (delete its results first)"));
+    if (!t.requires_grad()) return;
+    const auto index = t.device().index();
+    const auto here = c10::hip::getCurrentHIPStream(index).id(), standard = c10::hip::getDefaultHIPStream(index).id();
+    const std::shared_ptr<torch::autograd::Node> first = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
+    std::vector<torch::autograd::Node*> todo;
+    std::unordered_set<torch::autograd::Node*> seen;
+    auto meet = [&](torch::autograd::Node* n) {
+        if (n && seen.insert(n).second) todo.push_back(n);
+    };
+    meet(first.get());
+    while (!todo.empty()) {
+        torch::autograd::Node* const n = todo.back();
+        todo.pop_back();
+        const auto made_on = n->stream();
+        if (made_on && made_on->device() == t.device() && made_on->id() != here && (n == first.get() || made_on->id() == standard))
+            throw std::runtime_error(text(what, ": in a stream capture, while a graph behind its input made on another stream is alive (delete its results, or detach the input)"));
+        for (const auto& e : n->next_edges()) meet(e.function.get());
+    }
 }
 
 Tensor linear(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t N, int64_t K, const std::optional<Tensor>& bias) {

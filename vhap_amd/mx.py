@@ -123,7 +123,7 @@ def linear(x, w, bias=None):
     """y [..., N] = x [..., K] w^T (+ bias): w an MXTensor [N, K], x float32 / bfloat16 / float16, bias float32 [N]; y in x's type.  The products are exact,
     the sums are float32 in a fixed order, y is rounded once (float32 numbers below 2^-117 lose their last bits, those below 2^-126 may count as 0).  Gradients
     flow to x and bias (once: not twice differentiable; an input with a forward-mode tangent is refused).  In a stream capture, a differentiable call is refused while
-    a graph of the same leaf made on another stream is alive: its captured backward would end the process."""
+    a graph of the same input made on another stream is alive, or one made on the default stream anywhere behind it: its captured backward would end the process."""
     N, K = _matrix(w, "linear")
     return _lib.host().linear(x, w.codes, w.scales, N, K, bias)
 
