@@ -338,3 +338,52 @@ def test_a_capture_beside_an_eager_graph_behind_the_input():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(dx, 3 * mx.linear_input_grad(g, w)) and torch.equal(db, torch.autograd.grad(mx.linear(leaf.detach(), w, b1 := bias.detach().clone().requires_grad_()), b1, g)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("m,n,k", [(6200, 1000, 100), (6200, 1000, 128), (6145, 1023, 257), (12289, 513, 384), (70000, 65, 31)])
+def test_matmul_over_many_tiles(m, n, k, out):
+    """128 x 128 tiles: from 384 of them on"""
+    assert -(-m // 128) * -(-n // 128) >= 384
+    a, b, bias = random_mx(m, k, 1, lo=118, hi=127, garbage=True), random_mx(n, k, 2, lo=118, hi=127, garbage=True), randn((n,), 3)
+    A, B = values64(a), values64(b)
+    want, mags = A @ B.t(), A.abs() @ B.abs().t()
+    check_sum(mx.matmul(a, b, out_dtype=out), want, mags, k, out)
+    want, mags = want + bias.cpu().double(), mags + bias.abs().cpu().double()
+    check_sum(mx.matmul(a, b, bias, out_dtype=out), want, mags, k + 1, out)
+    check_sum(mx.matmul(a, b, bias, relu=True, out_dtype=out), want.clamp(min=0), mags, k + 1, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 40000, 200), (2, 40000, 200), (1, 40000, 300), (1, 40000, 401), (1, 32768, 512), (2, 32769, 129), (1, 40001, 100), (2, 40001, 128), (2, 300, 7)])
+def test_one_or_two_rows(m, n, k, dtype):
+    w = random_mx(n, k, m + n + k, garbage=True)
+    x, bias = randn((m, k), 1, dtype), randn((n,), 2)
+    W, X, b = values64(w), x.cpu().double(), bias.cpu().double()
+    check_sum(mx.linear(x, w), X @ W.t(), X.abs() @ W.abs().t(), k * PIECES[dtype], dtype)
+    check_sum(mx.linear(x, w, bias), X @ W.t() + b, X.abs() @ W.abs().t() + b.abs(), k * PIECES[dtype] + 1, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(1, 270001, 100), (1, 81000, 401), (2, 300000, 60)])
+def test_gradients_of_few_rows_against_a_large_matrix(m, n, k, dtype):
+    w, g = random_mx(n, k, 1, garbage=True), randn((m, n), 2, dtype)
+    W, G = w.dequantize().double(), g.double()                                   # (dequantize has its own tests)
+    check_sum(mx.linear_input_grad(g, w), (G @ W).cpu(), (G.abs() @ W.abs()).cpu(), n * PIECES[dtype] + 1024, dtype)
+
+
+@pytest.mark.gpu
+def test_quantize_past_32_bits_of_elements():
+    """rows x blocks x 4 past 2^31: the kernels' other index"""
+    rows = 2 ** 29 + 3
+    x = randn((1, 32), 1, torch.bfloat16)
+    q, one = mx.quantize(x.expand(rows, 32)), mx.quantize(x)
+    for at in range(0, rows, 2 ** 26):
+        assert bool((q.codes[at:at + 2 ** 26] == one.codes).all()) and bool((q.scales[at:at + 2 ** 26] == one.scales).all())
+    out, v = q.dequantize(torch.bfloat16), one.dequantize(torch.bfloat16)
+    del q
+    for at in range(0, rows, 2 ** 26):
+        assert bool((out[at:at + 2 ** 26] == v).all())
