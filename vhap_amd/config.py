@@ -35,7 +35,7 @@ class ModelConfig(Config):                                              # base.p
     remove_lip_inside: bool = False
     tex_resolution: int = 2048
     tex_painted: bool = True
-    tex_basis_format: str = "fp32"      # of the PCA texture space (tex_painted = False): "mxfp4" holds its basis in 4.25 bits an element (not in the reference)
+    tex_basis_format: str = "fp32"      # of the PCA texture space (tex_painted = False): "mxfp4" holds its basis in 4-bit floats, a sixth of the bytes (not in the reference)
     tex_extra: bool = True
     tex_clusters: Tuple[str, ...] = ("skin", "hair", "boundary", "lips_tight", "teeth", "sclerae", "irises")
     residual_tex: bool = True

@@ -10,7 +10,7 @@
 // (2 KB out of L2), with its first four units already on their way, so there is no third launch, no counter and no atomic -- the same call gives the same bits.
 // The sums are held in 64 bits: the square of an fp32 number is exact there, and no finite gradient overflows.  n is rounded to fp32 once; c is formed
 // from the 64-bit n and rounded to fp32 once.
-// 12.6 M fp32 gradients (50 MB): norm 11 us (4.5 TB/s: latency of the first loads and the waves' joins), scaling 18 us (101 MB, 5.6 TB/s), Adam 57 us (352 MB, 6.2 TB/s).
+// 12.6 M fp32 gradients (50 MB): norm 11 us (4.5 TB/s: a wave's six units are three rounds of loads one behind the other, 4 + 1 + 1, and the waves' joins), scaling 18 us (101 MB, 5.6 TB/s), Adam 57 us (352 MB, 6.2 TB/s).
 // Lists of at most ONE_BLOCK_UNITS units are one block's work in ONE launch (norm, barrier, scale): what counts there is the launches.
 #include "common.h"
 #include "elem8.h"

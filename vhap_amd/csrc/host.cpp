@@ -1,7 +1,7 @@
 // The host side of the calls whose device time is a few microseconds: walking a list of several hundred gradients, and the 4-bit products with their autograd node,
 // as an extension module over torch's C++ API.  It adds no arithmetic: checks, allocations, current stream, and the C ABI of libvhap_hip.so, whose entry points
 // it is handed as addresses (bind) by vhap_amd/_lib.py -- the library that the process already uses.
-// Why not in Python like the rest: reading five attributes each of 504 gradients and 504 results took 1.2 ms, six times the two launches they were read for; a Python
+// Why not in Python like the rest: reading five attributes each of 504 gradients and 504 results took 1.2 ms, forty times the two launches they were read for; a Python
 // autograd node's backward took about 100 us of host time around 40 us of kernels.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>

@@ -2,7 +2,7 @@
 //
 // A row of K numbers is cut into blocks of 32.  A block holds 32 codes of E2M1 -- +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, two a byte, the even element in the low
 // half -- and ONE byte b, the power of two 2^(b - 127) its codes are multiplied with (b = 255: the block is NaN).  codes [rows, 16 Kb], scales [rows, Kb],
-// Kb = ceil(K / 32): 0.53 bytes an element.
+// Kb = ceil(K / 32): 17 bytes a block, 0.53 an element of whole blocks (0.68 at K = 100, four blocks).
 //   quantise : b = max(0, exponent field of the block's largest magnitude - 2), so that the largest code lands in [4, 8); code = nearest of x / 2^(b - 127), halves
 //              to the even code, 6 at most.  A block of zeros has b = 0; a block with a NaN or an infinity has b = 255.
 //   linear   : y[m, n] = sum_k x[m, k] W[n, k] + bias[n]            W in 4 bits, x and y in fp32 / bf16 / fp16, sums in fp32
@@ -188,7 +188,7 @@ __device__ __forceinline__ void mx_fragments(const MxRaw8<DT>& r, bf16x8 (&out)[
 __device__ __forceinline__ int mx_left(long long at, long long end) { return at >= end ? 0 : end - at < 8 ? (int)(end - at) : 8; }
 
 // ---- quantise / dequantise: four lanes a block, eight elements a lane (16 or 32 contiguous bytes of x, one dword of codes) ----
-// Bound by HBM: 786432 x 100 fp32 -> codes 65 - 74 us (356 MB, 4.8 - 5.5 TB/s), codes -> bf16 38 - 41 us (199 MB, 5 TB/s); small ones by the launch (1023 x 257: 2.5 us each).
+// Bound by HBM: 786432 x 100 fp32 -> codes 65 - 74 us (368 MB, 5.0 - 5.7 TB/s), codes -> bf16 38 - 44 us (211 MB, 4.8 - 5.5 TB/s); small ones by the launch (1023 x 257: 2.5 us each).
 // Index: unsigned where rows x blocks x 4 is below 2^31, long long beyond (a 64-bit division is a hundred instructions: 1000 x 1000 bf16 there and back 4.6 us / 4.9).
 template <int DT, typename Index>
 __global__ __launch_bounds__(MX_T) void mx_quantize_kernel(const void* __restrict__ x, long long ldx, long long rows, int K, int Kb, uint8_t* __restrict__ codes,
@@ -277,7 +277,7 @@ __device__ __forceinline__ void mx_decode32(const u32x4& c, float scale, float (
 
 // One or two rows of x, K up to 128 KS: four lanes a row of W, a block of 32 each, against their 32 elements of x in registers -- 16 conversions and 32 M multiply-adds
 // for 16 bytes, under what memory delivers, and consecutive lanes read consecutive memory (in the matrix instruction's order they do not: see below).  1 x 786432 x 100 fp32:
-// 11.6 us for 48 MB (4.1 TB/s); what is left is the first loads' latency, behind x's way through LDS, and the tail.  768 to 2048 blocks differ by 4 %, and
+// 11.6 us for 60 MB (5.2 TB/s); what is left is the first loads' latency, behind x's way through LDS, and the tail.  768 to 2048 blocks differ by 4 %, and
 // the next rows read ahead of the products were no faster (12.4 us; 1 x 200000 x 400 20 instead of 13: their registers).
 template <int DT, int MM, int KS>
 __global__ __launch_bounds__(MX_T) void mx_linear_row_kernel(const MxLinear a) {
@@ -571,7 +571,7 @@ struct MxInputGrad {
 };
 
 // One row of g, fp32: per 16 rows of W a lane decodes one block of 32 (four lanes a row) and adds it, times g, to its 32 sums -- 16 conversions and 32 M
-// multiply-adds for 16 bytes, under what memory delivers.  1 x 786432 x 100: 11 us (45 MB, 4 TB/s), and 4 for the join.
+// multiply-adds for 16 bytes, under what memory delivers.  1 x 786432 x 100: 11 us (57 MB, 5.1 TB/s), and 4 for the join.
 __global__ __launch_bounds__(MX_T) void mx_input_grad_row_kernel(const MxInputGrad a) {
     __shared__ float red[MX_T / 64][32][64 + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = lane & 3, r = lane >> 2;
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(MX_T) void mx_input_grad_row_kernel(const MxInputGr
 // Any number of rows of g.  The sum runs along W's rows while its codes lie along K: a lane takes eight rows x eight elements of K (eight dwords), decodes them and turns
 // them in registers -- the bf16 pairs (k, k + 1) of two rows become the pairs (row, row + 1) of k and of k + 1 -- so that each of its eight k is one operand of a
 // matrix instruction over 32 rows.
-// 256 x 15429 x 400: 19 us in bf16 and 4 for the join (4 of them because half of g's rows begin between two dwords: 20 in all for 15428 columns); 64 x 786432 x 100: 39 us (142 MB, 3.6 TB/s).  A wave has few steps of 32
+// 256 x 15429 x 400: 19 us in bf16 and 4 for the join (4 of them because half of g's rows begin between two dwords: 20 in all for 15428 columns); 64 x 786432 x 100: 39 us (154 MB, 3.9 TB/s).  A wave has few steps of 32
 // rows there, about 1 us each: bound by latency and the vector unit's decoding and turning (80 instructions for 32 products); loads two or three steps ahead: 21 and 24 us
 // where one step was 20; eight waves a block: no faster.
 template <int DT, int CT>
@@ -1020,7 +1020,8 @@ struct GradPlan {
 GradPlan mx_grad_plan(long long M, long long N, int K, int dt) {
     GradPlan p;
     // one fp32 row against a large W is the vector unit's work (1 x 786432 x 100: 15.6 us, by the matrix instruction 26; 1 x 200000 x 400 15 / 27), anything else the matrix instruction's
-    // (1 x 200000 x 100: 12 us both; 1 x 15429 x 400 fp32 10 / 9, bf16 11 / 8)
+    // (1 x 200000 x 100: 12 us both; 1 x 15429 x 400 fp32 10 / 9, bf16 11 / 8).  It reads g in fp32: a 16-bit row is the matrix instruction's at any size (1 x 786432 x 100
+    // bf16 21 us, fp16 23; 1 x 200000 x 400 26)
     p.row = M == 1 && dt == VHAP_DTYPE_F32 && N * mx_kb(K) >= (1 << 20);
     p.ktiles = (K + 127) / 128;
     p.ct = M <= 16 ? 1 : M <= 32 || dt != VHAP_DTYPE_BF16 ? 2 : 4;                 // (64 rows in several pieces do not fit the registers)

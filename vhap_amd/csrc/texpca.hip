@@ -6,7 +6,7 @@
 // vhap_tex_prep_fwd.  HBM-bound: the basis is [S*S*3, n] floats = 315 MB at n = 100, read once forward and once backward:
 //   forward : one WAVE per row of the basis (lanes over the n coefficients, 400 contiguous bytes per row, DPP sum), four rows in flight;
 //             then one thread per texel of the T x T base (nearest source texel, channel swap, / 255, clamp)
-//   (vhap_tex_pca_mx4_*: the basis in microscaled 4-bit floats, 42 MB: the rows and d(code) are the 4-bit linear and its input's gradient, mx.hip)
+//   (vhap_tex_pca_mx4_*: the basis in microscaled 4-bit floats, 53 MB: the rows and d(code) are the 4-bit linear and its input's gradient, mx.hip)
 //   backward: per source texel the sum of d(base) over the texels it was copied to, masked by the clamp; then d(code) = basis^T g with
 //             one wave per run of rows, two coefficients per lane in registers, one atomic per coefficient and wave.
 #include "common.h"

