@@ -144,7 +144,7 @@ struct Place {
     struct Axis {
         int64_t c, most;
     };
-    int64_t lo, hi;
+    int64_t lo, hi, step = 0, run;            // the largest stride (0: none), and what lies within one
     std::vector<Axis> axes;
     explicit Place(const Tensor& t) {
         const int64_t size = (int64_t)t.element_size();
@@ -156,11 +156,21 @@ struct Place {
             axes.push_back({t.stride(d) * size, t.size(d) - 1});
             hi += axes.back().c * axes.back().most;
         }
+        run = hi - lo;
+        for (const Axis& a : axes)
+            if (a.c > step && a.most > 0) {
+                step = a.c;
+                run = hi - lo - a.c * a.most;
+            }
     }
-    // Nothing in common.  lo + sum c z = b.lo + sum c' z', with z' counted from its other end, is sum c z + sum c' (most' - z') = b.hi - 1 - lo: one sum of positive
-    // steps that reaches a given place, or does not.
+    // Nothing in common.  Columns of one matrix are told apart by where their runs lie in a row.  Otherwise: lo + sum c z = b.lo + sum c' z', with z' counted from its other
+    // end, is sum c z + sum c' (most' - z') = b.hi - 1 - lo: one sum of positive steps that reaches a given place, or does not.
     bool apart(const Place& b) const {
         if (hi <= b.lo || b.hi <= lo) return true;
+        if (step == b.step && step > 0) {
+            const int64_t to = ((b.lo - lo) % step + step) % step;
+            if (to >= run && to + b.run <= step) return true;
+        }
         std::vector<Axis> all(axes);
         all.insert(all.end(), b.axes.begin(), b.axes.end());
         int steps = 20000;
