@@ -387,3 +387,36 @@ def test_quantize_past_32_bits_of_elements():
     del q
     for at in range(0, rows, 2 ** 26):
         assert bool((out[at:at + 2 ** 26] == v).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limit", [None, 0.3])
+def test_state_loaded_into_an_optimiser_in_use(limit):
+    """the moments go where the kernels write them: into the tensors that a step has already been issued on"""
+    make = lambda: [torch.nn.Parameter(randn((300,), 1)), torch.nn.Parameter(randn((70, 1000), 2))]
+    a, b = make(), make()
+    oa, ob = NV.HipAdam(a, lr=1e-2, max_grad_norm=limit), NV.HipAdam(b, lr=1e-2, max_grad_norm=limit)
+
+    def step(ps, opt, k):
+        for i, p in enumerate(ps):
+            p.grad = randn(p.shape, 10 * k + i)
+        opt.step()
+    for k in range(3):
+        step(a, oa, k)
+        step(b, ob, k)
+    saved = {"state": {i: {n: t.clone() for n, t in s.items()} for i, s in oa.state_dict()["state"].items()}, "param_groups": oa.state_dict()["param_groups"]}
+    step(b, ob, 7)                                                               # b goes astray, and is taken back
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            q.copy_(p)
+    held = [ob.state[p]["exp_avg"].data_ptr() for p in b]
+    ob.load_state_dict(saved)
+    ob._step.copy_(oa._step)
+    assert [ob.state[p]["exp_avg"].data_ptr() for p in b] == held
+    for k in range(3, 5):
+        step(a, oa, k)
+        step(b, ob, k)
+        for p, q in zip(a, b):
+            assert torch.equal(p.detach(), q.detach())
+            for n in ("exp_avg", "exp_avg_sq"):
+                assert torch.equal(oa.state[p][n], ob.state[q][n])

@@ -481,6 +481,18 @@ class HipAdam(torch.optim.Optimizer):
         self._lr_host = None
         self.sync_lr()
 
+    def load_state_dict(self, state_dict):
+        """torch's; an optimiser in use keeps its moments' tensors (the kernels' pointer tables and captured steps hold their addresses) and takes the loaded values"""
+        held = {p: self.state[p] for p in self._tab["ps"]} if self._tab is not None else {}
+        super().load_state_dict(state_dict)
+        for p, st in held.items():
+            for name in ("exp_avg", "exp_avg_sq"):
+                if name in self.state[p]:
+                    st[name].copy_(self.state[p][name])
+                else:
+                    st[name].zero_()                              # (no step was counted for it)
+                self.state[p][name] = st[name]
+
     def lr_changed(self):
         return [float(g["lr"]) for g in self.param_groups] != self._lr_host
 
