@@ -420,3 +420,36 @@ def test_state_loaded_into_an_optimiser_in_use(limit):
             assert torch.equal(p.detach(), q.detach())
             for n in ("exp_avg", "exp_avg_sq"):
                 assert torch.equal(oa.state[p][n], ob.state[q][n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limit", [None, 0.3])
+@pytest.mark.parametrize("used", [False, True])
+def test_the_step_counter_is_part_of_the_state(limit, used):
+    """without it a resumed fit corrects its moments as if they had just begun"""
+    import copy
+    a, b = torch.nn.Parameter(randn((300,), 1)), torch.nn.Parameter(randn((300,), 1))
+    oa, ob = NV.HipAdam([a], lr=1e-2, max_grad_norm=limit), NV.HipAdam([b], lr=1e-2, max_grad_norm=limit)
+    assert ob.state_dict()["step"] == 0
+    if used:
+        b.grad = randn((300,), 9)
+        ob.step()
+    for k in range(3):
+        a.grad = randn((300,), 10 + k)
+        oa.step()
+    with torch.no_grad():
+        b.copy_(a)
+    saved = copy.deepcopy(oa.state_dict())
+    assert saved["step"] == 3
+    ob.load_state_dict(saved)
+    for k in range(2):
+        a.grad, b.grad = randn((300,), 20 + k), randn((300,), 20 + k)
+        oa.step()
+        ob.step()
+        assert torch.equal(a.detach(), b.detach()) and int(ob.step_count) == 4 + k
+    ob.load_state_dict({k: v for k, v in saved.items() if k != "step"})          # a state without one: the counter stays
+    assert int(ob.step_count) == 5
+    fresh = NV.HipAdam([b], lr=1e-2, max_grad_norm=limit)
+    fresh.load_state_dict(copy.deepcopy(saved))
+    fresh.reset_state()
+    assert fresh.state_dict()["step"] == 0 and not fresh.state_dict()["state"]

@@ -451,6 +451,7 @@ class HipAdam(torch.optim.Optimizer):
         self.grad_norm = None
         self._tab = None
         self._lr_host = None
+        self._first_step = 0                                      # what the counter starts from (load_state_dict)
 
     def _build(self):
         ps = [(gi, p) for gi, g in enumerate(self.param_groups) for p in g["params"]]
@@ -463,7 +464,7 @@ class HipAdam(torch.optim.Optimizer):
             st = self.state[p]
             if "exp_avg" not in st:
                 st["exp_avg"], st["exp_avg_sq"] = torch.zeros_like(p), torch.zeros_like(p)
-        self._step = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._step = torch.full((1,), self._first_step, dtype=torch.int32, device=dev)
         self._lr_dev = torch.zeros(len(self.param_groups), dtype=torch.float32, device=dev)
         n = len(ps)
         if self.max_grad_norm is not None:
@@ -481,6 +482,10 @@ class HipAdam(torch.optim.Optimizer):
         self._lr_host = None
         self.sync_lr()
 
+    def state_dict(self):
+        """torch's, with the step counter beside it as "step" (waits for the device)"""
+        return {**super().state_dict(), "step": self._first_step if self._tab is None else int(self._step)}
+
     def load_state_dict(self, state_dict):
         """torch's; an optimiser in use keeps its moments' tensors (the kernels' pointer tables and captured steps hold their addresses) and takes the loaded values"""
         held = {p: self.state[p] for p in self._tab["ps"]} if self._tab is not None else {}
@@ -492,6 +497,10 @@ class HipAdam(torch.optim.Optimizer):
                 else:
                     st[name].zero_()                              # (no step was counted for it)
                 self.state[p][name] = st[name]
+        if "step" in state_dict:
+            self._first_step = int(state_dict["step"])
+            if self._tab is not None:
+                self._step.fill_(self._first_step)
 
     def lr_changed(self):
         return [float(g["lr"]) for g in self.param_groups] != self._lr_host
@@ -510,6 +519,8 @@ class HipAdam(torch.optim.Optimizer):
     def reset_state(self, lr_scale_base=None):
         """Back to a freshly constructed optimiser: zero moments, step 0 (the reference builds a new Adam per optimize_stage call)."""
         if self._tab is None:
+            self.state.clear()                                    # (loaded, not yet used)
+            self._first_step = 0
             return
         for p in self._tab["ps"]:
             st = self.state[p]
